@@ -38,6 +38,13 @@ extern "C" {
 #define B2_SCALE_E4M3 0
 #define B2_SCALE_UE8M0 1
 
+/* activations of the product epilogues */
+#define B2_ACT_NONE 0
+#define B2_ACT_RELU 1
+#define B2_ACT_GELU 2      /* v * Phi(v)                                                       */
+#define B2_ACT_GELU_TANH 3 /* v / 2 * (1 + tanh(sqrt(2/pi) * (v + 0.044715 * v^3)))              */
+#define B2_ACT_SILU 4      /* v / (1 + exp(-v))                                                */
+
 /* op codes of b2_mufu_probe */
 #define B2_MUFU_RCP_FTZ 0   /* rcp.approx.ftz.f32   */
 #define B2_MUFU_RSQRT_FTZ 1 /* rsqrt.approx.ftz.f32 */
@@ -255,6 +262,105 @@ int b2_peer_close(void* ptr);
 int b2_nvfp4_gemm_allgather(const void* A, const void* B, const void* SFA, const void* SFB,
                             const float* alpha_dev, void* const* D_all, int world, int rank,
                             int M, int N, int K, void* stream);
+
+/*
+ * Block-scaled NVFP4 products with a fused epilogue.  No counterpart in the reference (its nvfp4_gemm stores
+ * alpha * A B^T); they stand beside b2_nvfp4_gemm and share its operand format.
+ *
+ * b2_nvfp4_gemm_epilogue:  D[M,N] = residual + act(alpha * A[M,K] * B[N,K]^T + bias)
+ *   A, B, SFA, SFB, alpha_dev   as b2_nvfp4_gemm
+ *   bias      [N] or NULL, residual [M,N] or NULL (may be D), D [M,N]: all of out_dtype, row-major, contiguous
+ *   activation  B2_ACT_*
+ * b2_nvfp4_grouped_gemm:  rows offsets[g] .. offsets[g+1] of D = act(alpha[g] * A * B[g]^T + bias[g])
+ *   A         uint8 [rows, K/2]; SFA: 128x4 tiles, group g from tile offsets[g] / 128 + g on
+ *             (b2_nvfp4_grouped_sf_bytes; what no row has may hold anything)
+ *   B         uint8 [groups, N, K/2]; SFB: ceil(N/128)*128 x K/16 bytes of 128x4 tiles per group
+ *   alpha_dev fp32 [groups]; offsets_dev int32 [groups + 1], ascending, read on the device (groups may be empty;
+ *             offsets that are not ascending or leave [0, rows] are clamped); bias [groups, N] or NULL
+ *   Rows of D in front of offsets[0] and from offsets[groups] on are left as they were.
+ * Sums, bias, activation and residual are fp32, with one rounding to the output.
+ * Requirements: K % 64 == 0, N % 8 == 0, rows >= 0 (0: nothing is launched), 1 to 384 groups, pointers 16-byte aligned
+ * (alpha, offsets 4-byte).  Where the padding rows or columns of the scale buffers lie, any bytes may stand.
+ * Nothing is allocated and no workspace is used: calls on different streams do not interfere.  The first call on a
+ * device sets a kernel attribute; make it before any stream capture.  Launch order as b2_nvfp4_gemm.
+ */
+int b2_nvfp4_gemm_epilogue(const void* A, const void* B, const void* SFA, const void* SFB, const float* alpha_dev,
+                           const void* bias, const void* residual, void* D, int M, int N, int K, int out_dtype,
+                           int activation, void* stream);
+int b2_nvfp4_grouped_gemm(const void* A, const void* B, const void* SFA, const void* SFB, const float* alpha_dev,
+                          const int32_t* offsets_dev, const void* bias, void* D, int rows, int groups, int N, int K,
+                          int out_dtype, int activation, void* stream);
+
+/* Kernel variant of the following two products' calls (-1: automatic): 0, 1 tiles of 32 rows x 64 columns (two MMA
+ * warps / two accumulators in turn), 2 128 x 64, 3 and 4 128 x 128 (two MMA warps / two accumulators), 5 a CTA pair
+ * with 256 x 256, 6 a CTA pair with 256 x 128.  Every variant takes every shape. */
+int b2_nvfp4_grouped_gemm_set_variant(int variant);
+
+/* Reads and clears the status words of the two products on the current device, as b2_nvfp4_gemm_status. */
+int b2_nvfp4_grouped_gemm_status(void* stream);
+
+/*
+ * NVFP4 quantizer with the grouped scale layout: row r of the output is row index[r] of the input (row r without
+ * index), quantized as b2_nvfp4_quantize does with the encode scale of r's group.
+ *   in [in_rows, k] fp16/bf16 ([in_rows, 2k] = [gate | up] with fuse_silu); index_dev int32 [rows] or NULL (an index
+ *   outside [0, in_rows) gives a row of zeros); offsets_dev int32 [groups + 1]; out uint8 [rows, k/2];
+ *   sf b2_nvfp4_grouped_sf_bytes(rows, groups, k) bytes, written only where rows are; gs_dev fp32 [groups]
+ * Rows from offsets[groups] on are left as they were.  Requirements: k % 64 == 0, rows >= 0, 1 to 384 groups,
+ * `in` 16-byte (32 for the wider loads), `out` 8-byte aligned.
+ */
+int b2_nvfp4_quantize_grouped(const void* in, const int32_t* index_dev, const int32_t* offsets_dev, void* out, void* sf,
+                              const float* gs_dev, int in_rows, int rows, int groups, int k, int in_dtype,
+                              int fuse_silu, void* stream);
+int64_t b2_nvfp4_grouped_sf_bytes(int rows, int groups, int k);
+
+/*
+ * Routing plan: assignment i (token i / topk, expert ids[i]) gets row position[i] of the rows sorted by expert, in
+ * order of i within an expert.  ids outside [0, experts) are dropped (position -1).
+ *   ids_dev int32 [tokens, topk]; offsets_dev int32 [experts + 1]; row_token_dev int32 [tokens * topk]: the token of a
+ *   row, -1 behind the last; position_dev int32 [tokens, topk].  1 to 384 experts.
+ */
+int b2_moe_plan(const int32_t* ids_dev, int32_t* offsets_dev, int32_t* row_token_dev, int32_t* position_dev, int tokens,
+                int topk, int experts, void* stream);
+
+/*
+ * out[t] = residual[t] + sum over k of weight[t,k] * y[position[t,k]], in order of k, fp32 with one rounding.
+ *   y [rows, n], residual [tokens, n] or NULL (may be out), out [tokens, n], all of dtype; position int32, weight fp32
+ *   [tokens, topk].  Positions outside [0, rows) add nothing.  n % 8 == 0, 16-byte aligned tensors.
+ */
+int b2_moe_combine(const void* y, const int32_t* position_dev, const float* weight_dev, const void* residual, void* out,
+                   int rows, int tokens, int topk, int n, int dtype, void* stream);
+
+/*
+ * Routed feed-forward: plan, quantize x per expert, product with W1 (uint8 [experts, 2 * inner, hidden/2], gate rows
+ * in front of up rows), SiLU(gate) * up quantized per expert, product with W2 (uint8 [experts, hidden, inner/2]),
+ * weighted sum per token.  Six launches on `stream`, each of the entry points above.
+ *   x, residual (or NULL), out [tokens, hidden] of dtype; alpha1, gs1, alpha2, gs2 fp32 [experts]: gs the encode scale of
+ *   the activations, alpha 1 / (gs * the weight's encode scale)
+ *   workspace  b2_moe_expert_ffn_workspace_bytes(...) bytes, 256-byte aligned; its contents need not be kept between
+ *              calls, and calls that may overlap (other streams, graphs replayed at once) need one each
+ * hidden and inner are multiples of 64.
+ */
+int b2_moe_expert_ffn(const void* x, const int32_t* ids_dev, const float* weight_dev, const void* W1, const void* SF1,
+                      const float* alpha1_dev, const float* gs1_dev, const void* W2, const void* SF2,
+                      const float* alpha2_dev, const float* gs2_dev, const void* residual, void* out, void* workspace,
+                      int64_t workspace_bytes, int tokens, int topk, int experts, int hidden, int inner, int dtype,
+                      void* stream);
+int64_t b2_moe_expert_ffn_workspace_bytes(int tokens, int topk, int experts, int hidden, int inner);
+
+/*
+ * The residual stream between two blocks:
+ *   u = x * rsqrt(mean(x^2) + eps) * w_post      (u = x when w_post is NULL)
+ *   h = residual_scale * residual + gate * u     (gate row t / rows_per_gate for row t; 1 when gate is NULL)
+ *   y = h * rsqrt(mean(h^2) + eps) * w_pre       (h as rounded to the input type)
+ * h goes to residual_out (may be `residual`), y to [M, H] of the input type or, with quantize, to packed E2M1
+ * uint8 [M, H/2] with one E4M3 scale per 16 values in sf: [M, H/16], or 128x4-swizzled (padding positions are left
+ * untouched).  x, residual, weights, gate [ceil(M / rows_per_gate), H] of in_dtype.
+ * Requirements: H % 16 == 0, 16 <= H <= 32768, 16-bit tensors 32-byte aligned.  gs_dev, sf only with quantize.
+ */
+int b2_gated_add_rmsnorm_fp4quant(const void* x, const void* residual, const void* w_post, const void* gate,
+                                  const void* w_pre, void* residual_out, void* y, void* sf, const float* gs_dev, int M,
+                                  int H, int rows_per_gate, float residual_scale, float eps, int in_dtype, int quantize,
+                                  int swizzled, void* stream);
 
 /*
  * In-kernel role timers of b2_nvfp4_gemm (observability; the reference's nearest analogue is the

@@ -1,0 +1,810 @@
+// Block-scaled NVFP4 products with a fused epilogue, dense and grouped by expert, for sm_100a:
+//
+//   D[r, :] = residual[r, :] + act(alpha[g] * A[r, :] B[g]^T + bias[g, :])        for the rows r of group g
+//
+// A [rows, K] and B [groups, N, K] are E2M1 with one E4M3 scale per 16 values along K; the sum is fp32 in tensor
+// memory, everything after it fp32 in registers, with one rounding to the 16-bit output.  The dense product
+// (b2_nvfp4_gemm_epilogue) is the grouped one with a single group that has all rows.  Groups are ragged: group g
+// has rows offsets[g] .. offsets[g+1] of A and D, read on the device, so a router's result is never waited for by
+// the host.  The 128-row tiles of A's scale factors start anew with every group: group g begins at tile
+// offsets[g] / 128 + g.  (The next group begins at or behind this one's last tile because
+// ceil(n / 128) <= floor((o + n) / 128) - floor(o / 128) + 1; no prefix sum is needed to find a row's scales.)
+// B's scale tiles are ceil(N / 128) per group.
+//
+// The K-slab pipeline is that of nvfp4_gemm.cu: operands by TMA into a ring of stages, scale factors through
+// registers into tensor memory, tcgen05.mma by one thread, an epilogue of eight warps.  What differs:
+//
+//   * the tile list is made on the device: one warp sums the groups' row tiles (a table in shared memory), every
+//     role finds (group, row tile, column tile) of its next work item there by bisection;
+//   * rows of a tile that belong to the next group are multiplied and dropped: a 32-row part of a tile is stored by
+//     the TMA where it lies inside the group, row by row where the group ends inside it;
+//   * K needs no multiple of the slab: the TMA fills operands and scales behind K with zeros; columns behind N are
+//     multiplied (zeros, or the next group's weights) and dropped;
+//   * 32-row tiles for groups of a few rows (AM = 32) may start in any quarter of a 128-row scale tile; the scale
+//     warps move that quarter to the first place;
+//   * with NACC == 2 the accumulator is double: the next tile is multiplied while the epilogue works.
+//
+// The residual is loaded into the registers that later hold the packed output, before the wait for the
+// accumulator: its latency hides behind the products and costs no register.
+#include <atomic>
+
+#include "nvfp4_tile.cuh"
+
+namespace b2 {
+namespace {
+
+constexpr int kGroupThreads = 640;  // 4 issuing warps, 2 x 4 scale warps, 8 epilogue warps
+constexpr int kMaxGroups = 384;     // bounds the tables in shared memory
+constexpr int kTableBytes = 2 * (kMaxGroups + 1) * 4;
+constexpr int kGWarpOperands = 0, kGWarpMma = 1, kGWarpScales = 2, kGWarpMma2 = 3, kGWarpScale0 = 4, kGWarpEpi0 = 12;
+
+struct GroupedParams {
+  const float* alpha;       // [groups]
+  const int32_t* offsets;   // [groups + 1], or null: one group with all rows
+  const uint16_t* bias;     // [groups, N] or null
+  const uint16_t* residual; // [rows, N] or null
+  uint16_t* D;              // [rows, N]
+  uint32_t* status;
+  int rows, groups, N;
+  int k_slabs;
+  int tiles_n, group_n;
+  int act;                  // B2_ACT_*
+  int fp16;                 // 16-bit type of bias, residual and D
+  uint64_t wait_budget_ns;
+};
+
+template <int CG, int BN, int STAGES, int TMA_OUT, int AM>
+struct GroupedLayout : SmemLayout<CG, BN, STAGES, TMA_OUT, AM> {
+  using Base = SmemLayout<CG, BN, STAGES, TMA_OUT, AM>;
+  static constexpr int kTable = Base::kRingBytes + Base::kBarrierBytes;
+  static constexpr int kAll = kTable + kTableBytes + 1024;  // + alignment slack
+  static_assert(kAll <= 227 * 1024, "shared memory budget");
+};
+
+struct Tile {
+  int group, first, last;  // the group and its rows
+  int tm, tn;
+};
+
+// Work item t -> its tile.  starts[g] is the number of row tiles in front of group g; among groups without rows,
+// which share a start, bisection ends at the last one, the one that has the tile.
+__device__ __forceinline__ Tile find_tile(const GroupedParams& p, const int* starts, const int* rows, int t) {
+  const int q = t / p.tiles_n;
+  int lo = 0, hi = p.groups;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (starts[mid] <= q) lo = mid;
+    else hi = mid;
+  }
+  Tile r;
+  r.group = lo;
+  r.first = rows[lo];
+  r.last = rows[lo + 1];
+  const int before = starts[lo];
+  tile_coords(t - before * p.tiles_n, starts[lo + 1] - before, p.tiles_n, p.group_n, r.tm, r.tn);
+  return r;
+}
+
+// v / (1 + 2^-(v (c1 + c2 v^2)) ): SiLU with c1 = log2 e, c2 = 0; GELU in its tanh form, since
+// (1 + tanh u) / 2 = 1 / (1 + e^-2u), with c1 = 2 log2 e sqrt(2/pi), c2 = 0.044715 c1.  MUFU 2^x and 1/x (relative
+// error about 2^-22); 2^-x runs to infinity for very negative v, the quotient to -0.
+__device__ __forceinline__ float gate_sigmoid(float v, float c1, float c2) {
+  const float e = ex2_approx_ftz(-v * fmaf(c2, v * v, c1));
+  return v * rcp_approx_ftz(1.0f + e);
+}
+// v Phi(v) with the upper tail of the normal distribution by Abramowitz & Stegun 7.1.26 (absolute error 1.5e-7):
+// erfc(z) = (a1 t + .. + a5 t^5) e^(-z^2), t = 1 / (1 + p z), z = |v| / sqrt 2.
+__device__ __forceinline__ float gelu_erf(float v) {
+  const float z = fabsf(v) * 0.70710678118654752f;
+  const float t = rcp_approx_ftz(fmaf(0.3275911f, z, 1.0f));
+  float poly = fmaf(1.061405429f, t, -1.453152027f);
+  poly = fmaf(poly, t, 1.421413741f);
+  poly = fmaf(poly, t, -0.284496736f);
+  poly = fmaf(poly, t, 0.254829592f);
+  const float half_tail = 0.5f * poly * t * ex2_approx_ftz(z * z * -1.4426950408889634f);
+  return v * (v >= 0.0f ? 1.0f - half_tail : half_tail);
+}
+
+__device__ __forceinline__ float2 unpack_pair(uint32_t w, bool fp16) {
+  const float2 h = unpack2<F16Tag>(w), b = unpack2<BF16Tag>(w);
+  return make_float2(fp16 ? h.x : b.x, fp16 ? h.y : b.y);
+}
+__device__ __forceinline__ uint32_t pack_pair(float x, float y, bool fp16) {
+  const uint32_t h = pack_from_f32<F16Tag>(x, y), b = pack_from_f32<BF16Tag>(x, y);
+  return fp16 ? h : b;
+}
+
+// Not the read-only path: the residual may be the output's own memory (every word is read before it is written, by
+// the thread that writes it).
+__device__ __forceinline__ uint4 load_residual(const uint16_t* p) {
+  uint4 r;
+  asm volatile("ld.global.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+  return r;
+}
+
+// 32 accumulator columns of one row -> 16 packed words.  `io` holds the residual on entry.
+__device__ __forceinline__ void finish32(const GroupedParams& p, uint32_t (&v)[32], uint32_t* io, const uint16_t* bias,
+                                         int col, float alpha) {
+  const bool fp16 = p.fp16 != 0;
+  float f[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(v[i]) * alpha;
+  if (bias) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      if (col + 8 * c < p.N) {  // N is a multiple of 8
+        const uint4 b = __ldg(reinterpret_cast<const uint4*>(bias + col + 8 * c));
+        const uint32_t w[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 x = unpack_pair(w[i], fp16);
+          f[8 * c + 2 * i] += x.x;
+          f[8 * c + 2 * i + 1] += x.y;
+        }
+      }
+    }
+  }
+  if (p.act == B2_ACT_SILU || p.act == B2_ACT_GELU_TANH) {
+    const float c1 = p.act == B2_ACT_SILU ? 1.4426950408889634f : 2.3022081983375f;
+    const float c2 = p.act == B2_ACT_SILU ? 0.0f : 0.10294324f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) f[i] = gate_sigmoid(f[i], c1, c2);
+  } else if (p.act == B2_ACT_GELU) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) f[i] = gelu_erf(f[i]);
+  } else if (p.act == B2_ACT_RELU) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) f[i] = f[i] < 0.0f ? 0.0f : f[i];  // a NaN stays one
+  }
+  if (p.residual) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float2 r = unpack_pair(io[i], fp16);
+      f[2 * i] += r.x;
+      f[2 * i + 1] += r.y;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) io[i] = pack_pair(f[2 * i], f[2 * i + 1], fp16);
+}
+
+// CG: CTAs of a tile (1 or 2).  BN: its columns.  AM: rows of A that one CTA loads and multiplies (the MMA reads 128;
+// what follows a shorter box in the stage only reaches accumulator rows that nobody reads).  MMAS: MMA-issuing warps
+// with an accumulator each, for a single tile per CTA (issuing is the limit there).  NACC: accumulators in turn, for many tiles.
+template <int CG, int BN, int STAGES, int TMA_OUT, int AM, int MMAS, int NACC>
+__global__ void __launch_bounds__(kGroupThreads, 1)
+    nvfp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                              const __grid_constant__ CUtensorMap map_sfa, const __grid_constant__ CUtensorMap map_sfb,
+                              const __grid_constant__ CUtensorMap map_d, const __grid_constant__ GroupedParams p) {
+  using L = GroupedLayout<CG, BN, STAGES, TMA_OUT, AM>;
+  static_assert(MMAS == 1 || (CG == 1 && TMA_OUT == 0), "the second MMA warp exists for single-CTA tiles");
+  static_assert(CG == 1 || AM == kBlockM, "pairs load all rows");
+  constexpr int kBM = AM * CG;                // rows of a tile
+  constexpr int kAccCols = BN * MMAS * NACC;  // accumulator columns in front of the stages' scale areas
+  static_assert(kAccCols + STAGES * L::kSfCols <= 512, "tensor memory budget");
+  constexpr int kTmemCols = 512;
+  constexpr uint32_t kIdesc = instr_desc(kBlockM * CG, BN);
+  constexpr uint32_t kOperandTx = static_cast<uint32_t>(L::kABytes + L::kBBytes) * CG;
+  constexpr uint32_t kScaleTx = static_cast<uint32_t>(L::kSfaBytes + L::kSfbBytes);
+  constexpr bool kWarpWide = CG == 2;  // issuing roles run as whole warps (see nvfp4_gemm.cu)
+
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
+  const uint32_t bar_base = smem_base + L::kRingBytes;
+  // The barriers of nvfp4_gemm.cu: full (operands landed and scales in tensor memory, on the pair's leader), sfload
+  // (scale blocks landed in shared memory), empty (the stage's MMAs retired); per accumulator full and empty.
+  auto full_bar = [&](int s) { return bar_base + 8u * s; };
+  auto sfload_bar = [&](int s) { return bar_base + 8u * (STAGES + s); };
+  auto empty_bar = [&](int s) { return bar_base + 8u * (2 * STAGES + s); };
+  auto acc_full_bar = [&](int a) { return bar_base + 8u * (3 * STAGES + a); };
+  auto acc_empty_bar = [&](int a) { return bar_base + 8u * (3 * STAGES + NACC + a); };
+  static_assert((3 * STAGES + 2 * NACC) * 8 + 16 <= L::kBarrierBytes, "barrier area");
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_gen + L::kRingBytes + 8 * (3 * STAGES + 2 * NACC));
+  volatile uint32_t* abort_flag = tmem_slot + 1;
+  int* starts = reinterpret_cast<int*>(smem_gen + L::kTable);  // [groups + 1] row tiles in front of a group
+  int* group_rows = starts + kMaxGroups + 1;                   // [groups + 1] first row of a group
+  const WaitCtx ctx{p.status, abort_flag, p.wait_budget_ns};
+
+  const int warp = kWarpWide ? __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0)
+                             : static_cast<int>(threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = CG == 2 ? __shfl_sync(0xffffffffu, cluster_ctarank(), 0) : 0u;
+  const bool leader = rank == 0;
+  const int unit = CG == 2 ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
+  const int num_units = CG == 2 ? static_cast<int>(gridDim.x >> 1) : static_cast<int>(gridDim.x);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(full_bar(s), 1 + 4 * CG);  // the producer's expect_tx arrive + one arrive per scale warp of the group
+      mbar_init(sfload_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int a = 0; a < NACC; ++a) {
+      mbar_init(acc_full_bar(a), MMAS);
+      mbar_init(acc_empty_bar(a), 8 * CG);  // one arrive per epilogue warp of every CTA in the group
+    }
+    *abort_flag = 0u;
+    fence_barrier_init();
+    prefetch_tmap(&map_a);
+    prefetch_tmap(&map_b);
+    prefetch_tmap(&map_sfa);
+    prefetch_tmap(&map_sfb);
+  }
+  if (warp == kGWarpMma) {
+    tmem_alloc<CG>(smem_u32(tmem_slot), kTmemCols);
+    tmem_relinquish<CG>();
+  }
+  // Dependent launch as in nvfp4_gemm.cu: nothing in front of this wait touches global memory.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (warp == kGWarpMma2) {
+    int tiles = 0;  // row tiles in front of the 32 groups of this step
+    for (int g0 = 0; g0 < p.groups; g0 += 32) {
+      const int g = g0 + lane;
+      int first = 0, last = 0;
+      if (g < p.groups) {
+        // Offsets that are not ascending or leave [0, rows] are brought back into it: no access leaves A or D.
+        if (p.offsets) {
+          first = min(max(__ldg(p.offsets + g), 0), p.rows);
+          last = min(max(__ldg(p.offsets + g + 1), first), p.rows);
+        } else {
+          last = p.rows;
+        }
+      }
+      const int mine = (last - first + kBM - 1) / kBM;
+      int sum = mine;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, sum, d);
+        if (lane >= d) sum += up;
+      }
+      if (g < p.groups) {
+        starts[g] = tiles + sum - mine;
+        group_rows[g] = first;
+        if (g == p.groups - 1) {
+          starts[g + 1] = tiles + sum;
+          group_rows[g + 1] = last;
+        }
+      }
+      tiles += __shfl_sync(0xffffffffu, sum, 31);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (CG == 2) cluster_sync_all();
+  tc_fence_after();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const uint32_t tmem_base = kWarpWide ? __shfl_sync(0xffffffffu, *tmem_slot, 0) : *tmem_slot;
+  const int num_tiles = starts[p.groups] * p.tiles_n;
+  const int k_slabs = p.k_slabs;
+
+  // The waits of the issuing roles: of the whole warp with one outcome, or of lane 0.
+  auto role_wait = [&](uint32_t bar, uint32_t phase, uint32_t code) {
+    const bool ok = wait_or_abort(bar, phase, ctx, code);
+    if constexpr (kWarpWide) return __all_sync(0xffffffffu, ok) != 0;
+    else return ok;
+  };
+  auto issues = [&] { return kWarpWide ? elect_one() : true; };
+
+  if (warp == kGWarpOperands) {
+    // ================= TMA producer of the operands =================
+    if (kWarpWide || lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool alive = true;
+      for (int t = unit; t < num_tiles && alive; t += num_units) {
+        const Tile tile = find_tile(p, starts, group_rows, t);
+        const int row_a = tile.first + tile.tm * kBM + static_cast<int>(rank) * kBlockM;
+        const int row_b = tile.group * p.N + tile.tn * BN + static_cast<int>(rank) * L::kBRows;
+        for (int ks = 0; ks < k_slabs; ++ks) {
+          if (!role_wait(empty_bar(stage), phase ^ 1u, 1u)) { alive = false; break; }
+          const uint32_t sbase = smem_base + stage * L::kStageBytes;
+          // operand bytes of both CTAs of a pair are counted on the leader's barrier
+          const uint32_t op_bar = CG == 2 ? mapa_shared(full_bar(stage), 0) : full_bar(stage);
+          if (issues()) {
+            if (leader) mbar_expect_tx(full_bar(stage), kOperandTx);
+            tma_load_2d<CG>(sbase, &map_a, ks * 128, row_a, op_bar);
+            tma_load_2d<CG>(sbase + L::kABytes, &map_b, ks * 128, row_b, op_bar);
+          }
+          if constexpr (kWarpWide) __syncwarp();
+          if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+        }
+      }
+    }
+  } else if (warp == kGWarpScales) {
+    // ================= TMA producer of the scale factors =================
+    if (kWarpWide || lane == 0) {
+      const int sfb_tiles = (p.N + 127) / 128;
+      int stage = 0;
+      uint32_t phase = 0;
+      bool alive = true;
+      for (int t = unit; t < num_tiles && alive; t += num_units) {
+        const Tile tile = find_tile(p, starts, group_rows, t);
+        const int sfa_tile = (tile.first >> 7) + tile.group + ((tile.tm * kBM) >> 7) + static_cast<int>(rank);
+        const int sfb_tile = tile.group * sfb_tiles + (tile.tn * BN) / 128;
+        for (int ks = 0; ks < k_slabs; ++ks) {
+          if (!role_wait(empty_bar(stage), phase ^ 1u, 1u)) { alive = false; break; }
+          const uint32_t sf_smem = smem_base + stage * L::kStageBytes + L::kABytes + L::kBBytes;
+          if (issues()) {
+            mbar_expect_tx(sfload_bar(stage), kScaleTx);
+            tma_load_3d<1>(sf_smem, &map_sfa, 0, ks * 4, sfa_tile, sfload_bar(stage));
+            tma_load_3d<1>(sf_smem + L::kSfaBytes, &map_sfb, 0, ks * 4, sfb_tile, sfload_bar(stage));
+          }
+          if constexpr (kWarpWide) __syncwarp();
+          if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+        }
+      }
+    }
+  } else if (warp == kGWarpMma || (MMAS == 2 && warp == kGWarpMma2)) {
+    // ================= MMA issuer(s), in the leader =================
+    // Issuer `me` takes the K slabs with index % MMAS == me and adds them up in its own columns.
+    const int me = warp == kGWarpMma ? 0 : 1;
+    if (leader && (kWarpWide || lane == 0)) {
+      bool alive = true;
+      int acc = 0;
+      uint32_t acc_phase = 0;
+      int slab0 = 0;  // slabs of the tiles that are done: the ring position of this tile's first slab
+      for (int t = unit; t < num_tiles && alive; t += num_units, slab0 += k_slabs) {
+        if (!role_wait(acc_empty_bar(acc), acc_phase ^ 1u, 2u)) break;
+        tc_fence_after();
+        // A 64-wide tile uses half of a 128-row scale chunk of B: the upper half starts two columns in.
+        uint32_t sfb_half = 0;
+        if constexpr (BN == 64) sfb_half = static_cast<uint32_t>(find_tile(p, starts, group_rows, t).tn & 1) * 2u;
+        const uint32_t acc_tmem = tmem_base + static_cast<uint32_t>((acc * MMAS + me) * BN);
+        int stage = (slab0 + me) % STAGES;
+        uint32_t phase = static_cast<uint32_t>((slab0 + me) / STAGES) & 1u;
+        bool polled = false;  // the poll issued with the previous slab found this slab's barrier complete
+        for (int ks = me; ks < k_slabs; ks += MMAS) {
+          if (!polled && !role_wait(full_bar(stage), phase, 3u)) { alive = false; break; }
+          tc_fence_after();
+          const uint32_t sbase = smem_base + stage * L::kStageBytes;
+          const uint32_t sf_tmem = tmem_base + kAccCols + stage * L::kSfCols;
+          const uint64_t a_desc = operand_desc(sbase), b_desc = operand_desc(sbase + L::kABytes);
+          int next_stage = stage + MMAS;
+          uint32_t next_phase = phase;
+          if (next_stage >= STAGES) { next_stage -= STAGES; next_phase ^= 1u; }
+          if constexpr (kWarpWide) {
+            if (elect_one()) {
+#pragma unroll
+              for (int kb = 0; kb < 4; ++kb)
+                tc_mma<CG>(acc_tmem, a_desc + 2 * kb, b_desc + 2 * kb, kIdesc, sf_tmem + kb * 4,
+                           sf_tmem + 16 + kb * 4 * L::kChunks + sfb_half, (ks >= MMAS || kb) ? 1u : 0u);
+              tc_commit_pair(empty_bar(stage));
+            }
+            __syncwarp();
+          } else {
+            const bool more = ks + MMAS < k_slabs;  // behind the last slab the poll asks this slab's own barrier
+            const uint32_t ok = tc_slab_and_poll_next<CG>(
+                acc_tmem, a_desc, b_desc, kIdesc, sf_tmem, sf_tmem + 16 + sfb_half, 4 * L::kChunks,
+                ks >= MMAS ? 1u : 0u, empty_bar(stage), full_bar(more ? next_stage : stage),
+                more ? next_phase : phase);
+            polled = more && ok != 0;
+          }
+          stage = next_stage;
+          phase = next_phase;
+        }
+        if (!alive) break;
+        if (issues()) {
+          if constexpr (CG == 2) tc_commit_pair(acc_full_bar(acc));
+          else tc_commit<CG>(acc_full_bar(acc));
+        }
+        if constexpr (kWarpWide) __syncwarp();
+        if (++acc == NACC) { acc = 0; acc_phase ^= 1u; }
+      }
+    }
+  } else if (warp >= kGWarpScale0 && warp < kGWarpEpi0) {
+    // ================= scale warps: shared memory -> registers -> tensor memory =================
+    // Layout and reasons as in nvfp4_gemm.cu.  Two sets of four warps, by the parity of the stage.
+    const int quarter = warp & 3;
+    const int set = (warp - kGWarpScale0) >> 2;
+    const int total_slabs = unit < num_tiles ? ((num_tiles - unit + num_units - 1) / num_units) * k_slabs : 0;
+    int tile_slabs = 0, t = unit;  // slabs left of the current tile, the next tile (AM == 32 only)
+    int part = 0;                  // the 32-row quarter of the scale tile that this tile's rows have
+    for (int n = 0; n < total_slabs; ++n) {
+      if constexpr (AM == 32) {
+        if (tile_slabs == 0) {
+          part = find_tile(p, starts, group_rows, t).tm & 3;
+          t += num_units;
+          tile_slabs = k_slabs;
+        }
+        --tile_slabs;
+      }
+      const int stage = n % STAGES;
+      if ((stage & 1) != set) continue;
+      const uint32_t phase = static_cast<uint32_t>(n / STAGES) & 1u;
+      if (!wait_or_abort(sfload_bar(stage), phase, ctx, 5u)) break;
+      const uint32_t sfa_smem = smem_base + stage * L::kStageBytes + L::kABytes + L::kBBytes + lane * 16;
+      const uint32_t sfb_smem = sfa_smem + L::kSfaBytes;
+      uint32_t a[16], b[16 * L::kChunks];
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb) lds128(sfa_smem + kb * 512, a + 4 * kb);
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+        for (int c = 0; c < L::kChunks; ++c) lds128(sfb_smem + (c * 4 + kb) * 512, b + 4 * (kb * L::kChunks + c));
+      if constexpr (AM == 32) {
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb) {
+          const uint32_t low = part & 1 ? a[4 * kb + 1] : a[4 * kb], high = part & 1 ? a[4 * kb + 3] : a[4 * kb + 2];
+          a[4 * kb] = part & 2 ? high : low;
+        }
+      }
+      const uint32_t dst = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + kAccCols + stage * L::kSfCols;
+      tmem_st_32x32_x16(dst, a);
+#pragma unroll
+      for (int c = 0; c < L::kChunks; ++c) tmem_st_32x32_x16(dst + 16 + 16 * c, b + 16 * c);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (leader) mbar_arrive_local(full_bar(stage));
+        else mbar_arrive_cluster_relaxed(mapa_shared(full_bar(stage), 0));
+      }
+    }
+  } else if (warp >= kGWarpEpi0) {
+    // ================= epilogue: 8 warps, lane quarter = warp & 3, column half = (warp - 12) / 4 ===========
+    constexpr int kHalf = BN / 2;
+    const int quarter = warp & 3;
+    const int half = (warp - kGWarpEpi0) >> 2;
+    const uint64_t store_policy = l2_policy_evict_first();
+    const bool two = MMAS == 2 && k_slabs > 1;  // a single slab leaves the second issuer without one
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    for (int t = unit; t < num_tiles; t += num_units) {
+      const Tile tile = find_tile(p, starts, group_rows, t);
+      const float alpha = __ldg(p.alpha + tile.group);
+      const int in_tile = static_cast<int>(rank) * kBlockM + quarter * 32;  // first row of this warp in the tile
+      const int row0 = tile.first + tile.tm * kBM + in_tile;
+      const int row = row0 + lane;
+      const int col0 = tile.tn * BN + half * kHalf;
+      const bool any = in_tile < kBM && row0 < tile.last && col0 < p.N;  // the same in the whole warp
+      const bool mine = any && row < tile.last;
+      const int64_t at = static_cast<int64_t>(row) * p.N + col0;
+      const uint16_t* bias = p.bias ? p.bias + static_cast<int64_t>(tile.group) * p.N : nullptr;
+      uint32_t packed[kHalf / 2];
+      if (p.residual) {
+#pragma unroll
+        for (int i = 0; i < kHalf / 8; ++i) {
+          uint4 r = make_uint4(0u, 0u, 0u, 0u);
+          if (mine && col0 + 8 * i < p.N) r = load_residual(p.residual + at + 8 * i);
+          packed[4 * i] = r.x;
+          packed[4 * i + 1] = r.y;
+          packed[4 * i + 2] = r.z;
+          packed[4 * i + 3] = r.w;
+        }
+      }
+      if (!wait_or_abort(acc_full_bar(acc), acc_phase, ctx, 4u)) break;
+      tc_fence_after();
+      if (any) {
+        const uint32_t acc_tmem = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
+                                  static_cast<uint32_t>(acc * MMAS * BN + half * kHalf);
+#pragma unroll
+        for (int c0 = 0; c0 < kHalf; c0 += 32) {
+          uint32_t v[32];
+          tmem_ld_32x32(acc_tmem + c0, v);
+          if constexpr (MMAS == 2) {
+            if (two) {
+              uint32_t v2[32];
+              tmem_ld_32x32(acc_tmem + BN + c0, v2);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) + __uint_as_float(v2[i]));
+            }
+          }
+          tmem_ld_wait();
+          finish32(p, v, packed + c0 / 2, bias, col0 + c0, alpha);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (leader) mbar_arrive_local(acc_empty_bar(acc));
+        else mbar_arrive_cluster_relaxed(mapa_shared(acc_empty_bar(acc), 0));
+      }
+      if (++acc == NACC) { acc = 0; acc_phase ^= 1u; }
+      if (!any) continue;
+      // The TMA clips rows behind the last row and columns behind N, but knows nothing of groups.
+      if (TMA_OUT > 0 && (row0 + 32 <= tile.last || tile.last == p.rows)) {
+        if constexpr (TMA_OUT > 0) {
+          constexpr int kSubs = kHalf / 64;
+          const uint32_t staging = smem_base + STAGES * L::kStageBytes +
+                                   static_cast<uint32_t>(warp - kGWarpEpi0) * TMA_OUT * 4096u;
+#pragma unroll
+          for (int sub = 0; sub < kSubs; ++sub) {
+            if (sub % TMA_OUT == 0) {
+              if (lane == 0) bulk_wait_read_all();  // earlier stores have read the staging
+              __syncwarp();
+            }
+            const uint32_t buf = staging + (sub % TMA_OUT) * 4096u;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const uint32_t chunk = static_cast<uint32_t>(j) ^ (lane & 7u);
+              sts128(buf + lane * 128u + chunk * 16u, packed[sub * 32 + 4 * j], packed[sub * 32 + 4 * j + 1],
+                     packed[sub * 32 + 4 * j + 2], packed[sub * 32 + 4 * j + 3]);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              if (col0 + sub * 64 < p.N) tma_store_2d(&map_d, buf, col0 + sub * 64, row0, store_policy);
+              bulk_commit();
+            }
+          }
+        }
+      } else if (mine) {
+        uint4* dst = reinterpret_cast<uint4*>(p.D + at);
+#pragma unroll
+        for (int i = 0; i < kHalf / 8; ++i)
+          if (col0 + 8 * i < p.N)
+            dst[i] = make_uint4(packed[4 * i], packed[4 * i + 1], packed[4 * i + 2], packed[4 * i + 3]);
+      }
+    }
+    if constexpr (TMA_OUT > 0) {
+      if (lane == 0) bulk_wait_all();  // every store has left shared memory and is written
+    }
+  }
+
+  // ---- teardown: nobody leaves while a peer may still signal into this CTA ----
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    // give copies that may still be in flight time to land before shared memory is released
+    for (int i = 0; i < 64; ++i) __nanosleep(2000);
+  }
+  if constexpr (CG == 2) cluster_sync_all();
+  if (warp == kGWarpMma) {
+    tc_fence_after();
+    tmem_dealloc<CG>(tmem_base, kTmemCols);
+  }
+}
+
+// ---- host ----------------------------------------------------------------------------------------
+struct GroupedCall {
+  const void *A, *B, *SFA, *SFB;
+  int sfa_tiles;  // 128-row tiles of A's scale buffer
+  int K;
+  GroupedParams p;
+  const char* who;
+};
+
+template <int CG, int BN, int STAGES, int TMA_OUT, int AM, int MMAS, int NACC>
+int launch_grouped(const GroupedCall& c, cudaStream_t stream) {
+  using L = GroupedLayout<CG, BN, STAGES, TMA_OUT, AM>;
+  constexpr int kBM = AM * CG;
+  auto kernel = nvfp4_grouped_gemm_kernel<CG, BN, STAGES, TMA_OUT, AM, MMAS, NACC>;
+  GroupedParams p = c.p;
+  CUtensorMap map_a, map_b, map_sfa, map_sfb, map_d = {};
+  if (int rc = encode_operand_map(&map_a, c.A, p.rows, c.K, AM)) return rc;
+  if (int rc = encode_operand_map(&map_b, c.B, p.groups * p.N, c.K, L::kBRows)) return rc;
+  if (int rc = encode_scale_map(&map_sfa, c.SFA, c.sfa_tiles * 128, c.K, 1)) return rc;
+  if (int rc = encode_scale_map(&map_sfb, c.SFB, p.groups * ((p.N + 127) / 128) * 128, c.K, L::kChunks)) return rc;
+  if (TMA_OUT > 0) {
+    if (int rc = encode_output_map(&map_d, p.D, p.rows, p.N)) return rc;
+  }
+  p.k_slabs = (c.K + kBlockK - 1) / kBlockK;
+  p.tiles_n = (p.N + BN - 1) / BN;
+  p.group_n = 8;
+  const int sms = device_sm_count();
+  if (sms <= 0) return B2_ERR_CUDA;
+  // The most row tiles that the groups can have; for one group that is their number.
+  const int64_t tiles_m = p.offsets ? p.rows / kBM + static_cast<int64_t>(p.groups < p.rows ? p.groups : p.rows)
+                                    : (p.rows + kBM - 1) / kBM;
+  const int64_t tiles = tiles_m * p.tiles_n;
+  if (tiles > 0x3fffffff) {
+    set_error("%s: %lld tiles exceed the tile list's range", c.who, static_cast<long long>(tiles));
+    return B2_ERR_INVALID_ARGUMENT;
+  }
+  // As many persistent CTAs (pairs) as finish the tiles in the fewest rounds, and no more.
+  const int64_t rounds = (tiles + sms / CG - 1) / (sms / CG);
+  const int units = static_cast<int>((tiles + rounds - 1) / rounds);
+
+  {
+    static std::atomic<bool> configured[64] = {};  // per instantiation; setting it twice does no harm
+    int dev = 0;
+    B2_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !configured[dev].load(std::memory_order_acquire)) {
+      B2_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAll));
+      if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
+    }
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(units * CG);
+  cfg.blockDim = dim3(kGroupThreads);
+  cfg.dynamicSmemBytes = L::kAll;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  cfg.attrs = attr;
+  if (CG == 2) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = 2;
+    attr[cfg.numAttrs].val.clusterDim.y = 1;
+    attr[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
+  attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+  ++cfg.numAttrs;
+  B2_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, map_a, map_b, map_sfa, map_sfb, map_d, p));
+  return B2_OK;
+}
+
+// Status words of these launches: part of the library image, so that no call allocates.
+static __device__ uint32_t g_grouped_status[64];
+
+int grouped_status_words(uint32_t** out) {
+  static std::atomic<uint32_t*> cache[64] = {};
+  int dev = 0;
+  B2_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64) {
+    set_error("device ordinal %d out of range", dev);
+    return B2_ERR_CUDA;
+  }
+  uint32_t* words = cache[dev].load(std::memory_order_acquire);
+  if (!words) {
+    void* ptr = nullptr;
+    B2_CUDA_TRY(cudaGetSymbolAddress(&ptr, g_grouped_status));
+    words = static_cast<uint32_t*>(ptr);
+    cache[dev].store(words, std::memory_order_release);
+  }
+  *out = words;
+  return B2_OK;
+}
+
+std::atomic<int> g_grouped_variant{-1};  // test hook: -1 = automatic
+
+// The kernel for `rows` rows in `groups` groups (numbering of b2_nvfp4_grouped_gemm_set_variant).
+int choose_grouped_variant(int rows, int groups, int N, int sms) {
+  const int64_t mean = (static_cast<int64_t>(rows) + groups - 1) / groups;
+  if (mean <= 32) return groups == 1 && (N + 63) / 64 <= sms ? 0 : 1;
+  if (groups == 1 && rows <= 128 && (N + 63) / 64 <= sms) return 2;
+  const int64_t tiles = ((mean + 127) / 128) * groups * ((N + 127) / 128);
+  if (groups == 1 && tiles <= sms) return 3;
+  if (mean <= 128) return 4;
+  if (groups == 1) {
+    const int64_t pairs = (mean + 255) / 256 * ((N + 255) / 256);
+    return pairs * 2 <= sms / 2 ? 6 : 5;
+  }
+  return 5;
+}
+
+int run_grouped(const GroupedCall& c, cudaStream_t s) {
+  const int sms = device_sm_count();
+  if (sms <= 0) return B2_ERR_CUDA;
+  int variant = g_grouped_variant.load(std::memory_order_relaxed);
+  if (variant < 0) variant = choose_grouped_variant(c.p.rows, c.p.groups, c.p.N, sms);
+  switch (variant) {
+    case 0: return launch_grouped<1, 64, 11, 0, 32, 2, 1>(c, s);
+    case 1: return launch_grouped<1, 64, 11, 0, 32, 1, 2>(c, s);
+    case 2: return launch_grouped<1, 64, 7, 0, 128, 2, 1>(c, s);
+    case 3: return launch_grouped<1, 128, 6, 0, 128, 2, 1>(c, s);
+    case 4: return launch_grouped<1, 128, 6, 0, 128, 1, 2>(c, s);
+    case 5: return launch_grouped<2, 256, 5, 1, 128, 1, 1>(c, s);
+    default: return launch_grouped<2, 128, 6, 1, 128, 1, 2>(c, s);
+  }
+}
+
+// The checks that the dense and the grouped entry point share.
+int check_product(const GroupedCall& c, int out_dtype) {
+  const GroupedParams& p = c.p;
+  if (p.rows < 0 || p.N < 1 || c.K < 1 || p.N % 8 != 0 || c.K % 64 != 0) {
+    set_error("%s: %d rows, N=%d, K=%d: need rows >= 0, N %% 8 == 0, K %% 64 == 0", c.who, p.rows, p.N, c.K);
+    return B2_ERR_INVALID_ARGUMENT;
+  }
+  if (p.groups < 1 || p.groups > kMaxGroups || static_cast<int64_t>(p.groups) * ((p.N + 127) / 128 * 128) > 0x7fffffffll ||
+      p.rows > 0x7fffffff - 512) {
+    set_error("%s: %d groups of N=%d with %d rows: need 1 to %d groups, groups * N and rows below 2^31", c.who,
+              p.groups, p.N, p.rows, kMaxGroups);
+    return B2_ERR_INVALID_ARGUMENT;
+  }
+  if (out_dtype != B2_DTYPE_F16 && out_dtype != B2_DTYPE_BF16) {
+    set_error("%s: unsupported out_dtype %d", c.who, out_dtype);
+    return B2_ERR_INVALID_ARGUMENT;
+  }
+  if (p.act < B2_ACT_NONE || p.act > B2_ACT_SILU) {
+    set_error("%s: unknown activation %d", c.who, p.act);
+    return B2_ERR_INVALID_ARGUMENT;
+  }
+  if (p.rows == 0) return B2_OK;
+  if (!c.A || !c.B || !c.SFA || !c.SFB || !p.alpha || !p.D) {
+    set_error("%s: null pointer argument", c.who);
+    return B2_ERR_INVALID_ARGUMENT;
+  }
+  const uintptr_t all = reinterpret_cast<uintptr_t>(c.A) | reinterpret_cast<uintptr_t>(c.B) |
+                        reinterpret_cast<uintptr_t>(c.SFA) | reinterpret_cast<uintptr_t>(c.SFB) |
+                        reinterpret_cast<uintptr_t>(p.D) | reinterpret_cast<uintptr_t>(p.bias) |
+                        reinterpret_cast<uintptr_t>(p.residual);
+  if ((all & 15) || ((reinterpret_cast<uintptr_t>(p.alpha) | reinterpret_cast<uintptr_t>(p.offsets)) & 3)) {
+    set_error("%s: operands, scales, bias, residual and output must be 16-byte aligned, alpha and offsets 4-byte", c.who);
+    return B2_ERR_INVALID_ARGUMENT;
+  }
+  if (!encode_tiled_fn()) {
+    set_error("%s: cuTensorMapEncodeTiled is not available from this driver", c.who);
+    return B2_ERR_CUDA;
+  }
+  return B2_OK;
+}
+
+}  // namespace
+}  // namespace b2
+
+extern "C" int b2_nvfp4_gemm_epilogue(const void* A, const void* B, const void* SFA, const void* SFB,
+                                      const float* alpha_dev, const void* bias, const void* residual, void* D, int M,
+                                      int N, int K, int out_dtype, int activation, void* stream) {
+  using namespace b2;
+  GroupedCall c = {};
+  c.who = "b2_nvfp4_gemm_epilogue";
+  c.A = A;
+  c.B = B;
+  c.SFA = SFA;
+  c.SFB = SFB;
+  c.K = K;
+  c.p.alpha = alpha_dev;
+  c.p.bias = static_cast<const uint16_t*>(bias);
+  c.p.residual = static_cast<const uint16_t*>(residual);
+  c.p.D = static_cast<uint16_t*>(D);
+  c.p.rows = M;
+  c.p.groups = 1;
+  c.p.N = N;
+  c.p.act = activation;
+  c.p.fp16 = out_dtype == B2_DTYPE_F16;
+  c.p.wait_budget_ns = kWaitBudgetNs;
+  if (int rc = check_product(c, out_dtype)) return rc;
+  if (M == 0) return B2_OK;
+  c.sfa_tiles = (M + 127) / 128;
+  if (int rc = grouped_status_words(&c.p.status)) return rc;
+  return run_grouped(c, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int b2_nvfp4_grouped_gemm(const void* A, const void* B, const void* SFA, const void* SFB,
+                                     const float* alpha_dev, const int32_t* offsets_dev, const void* bias, void* D,
+                                     int rows, int groups, int N, int K, int out_dtype, int activation, void* stream) {
+  using namespace b2;
+  GroupedCall c = {};
+  c.who = "b2_nvfp4_grouped_gemm";
+  c.A = A;
+  c.B = B;
+  c.SFA = SFA;
+  c.SFB = SFB;
+  c.K = K;
+  c.p.alpha = alpha_dev;
+  c.p.offsets = offsets_dev;
+  c.p.bias = static_cast<const uint16_t*>(bias);
+  c.p.D = static_cast<uint16_t*>(D);
+  c.p.rows = rows;
+  c.p.groups = groups;
+  c.p.N = N;
+  c.p.act = activation;
+  c.p.fp16 = out_dtype == B2_DTYPE_F16;
+  c.p.wait_budget_ns = kWaitBudgetNs;
+  if (int rc = check_product(c, out_dtype)) return rc;
+  if (rows == 0) return B2_OK;
+  if (!offsets_dev) {
+    set_error("b2_nvfp4_grouped_gemm: null pointer argument");
+    return B2_ERR_INVALID_ARGUMENT;
+  }
+  c.sfa_tiles = rows / 128 + groups;
+  if (int rc = grouped_status_words(&c.p.status)) return rc;
+  return run_grouped(c, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int b2_nvfp4_grouped_gemm_set_variant(int variant) {
+  if (variant < -1 || variant > 6) {
+    b2::set_error("b2_nvfp4_grouped_gemm_set_variant: unknown variant %d", variant);
+    return B2_ERR_INVALID_ARGUMENT;
+  }
+  b2::g_grouped_variant.store(variant, std::memory_order_relaxed);
+  return B2_OK;
+}
+
+extern "C" int b2_nvfp4_grouped_gemm_status(void* stream) {
+  using namespace b2;
+  uint32_t* status = nullptr;
+  if (int rc = grouped_status_words(&status)) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  uint32_t host[2] = {0, 0};
+  B2_CUDA_TRY(cudaMemcpyAsync(host, status, sizeof(host), cudaMemcpyDeviceToHost, s));
+  B2_CUDA_TRY(cudaStreamSynchronize(s));
+  if (host[0] == 0) return B2_OK;
+  B2_CUDA_TRY(cudaMemsetAsync(status, 0, sizeof(host), s));
+  set_error("b2_nvfp4_grouped_gemm: bounded wait %u expired in CTA %u", host[0], host[1]);
+  return B2_ERR_DEVICE_TIMEOUT;
+}

@@ -56,7 +56,7 @@ def unpack_e2m1(packed):
     import torch
 
     m = packed.shape[0]
-    nibbles = torch.stack((packed & 0x0F, packed >> 4), dim=-1).reshape(m, -1).long()
+    nibbles = torch.stack((packed & 0x0F, packed >> 4), dim=-1).reshape(m, 2 * packed.shape[1]).long()
     table = torch.tensor(E2M1_TABLE, device=packed.device, dtype=torch.float32)
     return table[nibbles]
 
@@ -103,6 +103,57 @@ def dequantized_matmul_fp32(A_fp4, B_fp4, A_sf, B_sf, alpha: float, *, row_chunk
     finally:
         torch.backends.cuda.matmul.allow_tf32 = tf32
         torch.set_float32_matmul_precision(precision)
+
+
+def require_tensor(name: str, tensor, dtype, shape) -> None:
+    """ValueError unless `tensor` has this dtype (a torch dtype or its name) and this shape (an int: that many elements)."""
+    import torch
+
+    want = getattr(torch, dtype) if isinstance(dtype, str) else dtype
+    if not isinstance(tensor, torch.Tensor):
+        raise ValueError(f"{name} must be a tensor, got {type(tensor).__name__}")
+    if tensor.dtype != want:
+        raise ValueError(f"{name} must be {want}, got {tensor.dtype}")
+    if isinstance(shape, int):
+        if tensor.numel() != shape:
+            raise ValueError(f"{name} must have {shape} elements, got {tensor.numel()}")
+    elif tuple(tensor.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(tensor.shape)}")
+
+
+def grouped_sf_numel(rows: int, groups: int, k: int) -> int:
+    """Bytes of the grouped 128x4 scale layout: group g begins at tile offsets[g] // 128 + g."""
+    return (rows // 128 + groups) * 128 * (k // 16)
+
+
+def grouped_sf_rows(offsets, rows: int):
+    """(group of every row, its row in the grouped scale tiles); rows outside every group are not meaningful."""
+    import torch
+
+    r = torch.arange(rows, device=offsets.device)
+    ends = offsets.long()
+    group = (torch.searchsorted(ends, r, right=True) - 1).clamp(0, offsets.numel() - 2)
+    first = ends[group]
+    return group, (first // 128 + group) * 128 + r - first
+
+
+def dequantize_rows(packed, sf, sf_rows):
+    """float64 values of packed rows whose scales are at the rows `sf_rows` of 128x4 tiles (no encode scale)."""
+    import torch
+
+    cols = packed.shape[1] // 8
+    tile_rows = sf.numel() // padded_sf_cols(cols)
+    scales = logical_scale_bytes(sf, tile_rows, cols, "128x4")[sf_rows].view(torch.float8_e4m3fn).double()
+    values = unpack_e2m1(packed).double()
+    return (values.view(values.shape[0], cols, 16) * scales[..., None]).reshape(values.shape)
+
+
+def activation(v, name: str):
+    """The epilogue's activations in the type of `v`."""
+    from torch.nn import functional as F
+
+    return {"none": lambda: v, "relu": lambda: F.relu(v), "gelu": lambda: F.gelu(v),
+            "gelu_tanh": lambda: F.gelu(v, approximate="tanh"), "silu": lambda: F.silu(v)}[name]()
 
 
 def padding_mask(m: int, sf_cols: int, layout: str, device):

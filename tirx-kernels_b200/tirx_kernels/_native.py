@@ -13,6 +13,8 @@ from pathlib import Path
 DTYPE_CODES = {"float16": 0, "bfloat16": 1}
 SF_LAYOUT_CODES = {"linear": 0, "128x4": 1, "8x4": 2}
 SCALE_FORMAT_CODES = {"e4m3": 0, "ue8m0": 1}
+ACTIVATION_CODES = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+MAX_GROUPS = 384  # groups (experts) of one grouped launch
 MUFU_OPS = {"rcp_ftz": 0, "rsqrt_ftz": 1, "lg2": 2, "ex2": 3, "ex2_ftz": 4,
             # the quantizer's SiLU as its kernel computes it / with div.rn.f32 throughout
             "silu": 5, "silu_div_rn": 6}
@@ -39,6 +41,17 @@ MAIN_SIGNATURES = {
     "b2_nvfp4_gemm_small_m_noalloc": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp]),
     "b2_nvfp4_gemm_status": (_i, [_vp]),
     "b2_nvfp4_gemm_small_m_noalloc_status": (_i, [_vp]),
+    "b2_nvfp4_gemm_epilogue": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
+    "b2_nvfp4_grouped_gemm": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp]),
+    "b2_nvfp4_grouped_gemm_set_variant": (_i, [_i]),
+    "b2_nvfp4_grouped_gemm_status": (_i, [_vp]),
+    "b2_nvfp4_quantize_grouped": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp]),
+    "b2_nvfp4_grouped_sf_bytes": (_i64, [_i, _i, _i]),
+    "b2_moe_plan": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _vp]),
+    "b2_moe_combine": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
+    "b2_moe_expert_ffn": (_i, [_vp] * 14 + [_i64] + [_i] * 6 + [_vp]),
+    "b2_moe_expert_ffn_workspace_bytes": (_i64, [_i, _i, _i, _i, _i]),
+    "b2_gated_add_rmsnorm_fp4quant": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _f, _f, _i, _i, _i, _vp]),
     "b2_nvfp4_gemm_set_wait_budget_ms": (_i, [_i]),
     "b2_nvfp4_gemm_inject_test_fault": (_i, [_i]),
     "b2_nvfp4_gemm_set_variant": (_i, [_i]),
@@ -213,6 +226,113 @@ def nvfp4_gemm_small_m_noalloc(A, B, SFA, SFB, alpha, D, M: int, N: int, K: int)
         lib().b2_nvfp4_gemm_small_m_noalloc(_ptr(A), _ptr(B), _ptr(SFA), _ptr(SFB), _ptr(alpha), _ptr(D),
                                             M, N, K, current_stream_ptr()),
         "b2_nvfp4_gemm_small_m_noalloc",
+    )
+
+
+def _require_here(*tensors) -> None:
+    """CUDA, contiguous, and on the current device, whose stream the launch goes to; None is an absent argument."""
+    import torch
+
+    present = [t for t in tensors if t is not None]
+    _require_cuda(*present)
+    device = torch.cuda.current_device()
+    for t in present:
+        if t.device.index != device:
+            raise ValueError(f"tensor on {t.device}, but the current device is cuda:{device}")
+
+
+def _ptr_or_null(tensor) -> int | None:
+    return None if tensor is None else tensor.data_ptr()
+
+
+def nvfp4_gemm_epilogue(A, B, SFA, SFB, alpha, bias, residual, D, M: int, N: int, K: int, out_dtype: str,
+                        activation: str = "none") -> None:
+    """D = residual + act(alpha * A B^T + bias); bias and residual may be None."""
+    _require_here(A, B, SFA, SFB, alpha, bias, residual, D)
+    check(
+        lib().b2_nvfp4_gemm_epilogue(_ptr(A), _ptr(B), _ptr(SFA), _ptr(SFB), _ptr(alpha), _ptr_or_null(bias),
+                                     _ptr_or_null(residual), _ptr(D), M, N, K, DTYPE_CODES[out_dtype],
+                                     ACTIVATION_CODES[activation], current_stream_ptr()),
+        "b2_nvfp4_gemm_epilogue",
+    )
+
+
+def nvfp4_grouped_gemm(A, B, SFA, SFB, alpha, offsets, bias, D, rows: int, groups: int, N: int, K: int, out_dtype: str,
+                       activation: str = "none") -> None:
+    """Rows offsets[g]..offsets[g+1] of D = act(alpha[g] * A B[g]^T + bias[g]); bias may be None."""
+    _require_here(A, B, SFA, SFB, alpha, offsets, bias, D)
+    check(
+        lib().b2_nvfp4_grouped_gemm(_ptr(A), _ptr(B), _ptr(SFA), _ptr(SFB), _ptr(alpha), _ptr(offsets),
+                                    _ptr_or_null(bias), _ptr(D), rows, groups, N, K, DTYPE_CODES[out_dtype],
+                                    ACTIVATION_CODES[activation], current_stream_ptr()),
+        "b2_nvfp4_grouped_gemm",
+    )
+
+
+def nvfp4_grouped_gemm_set_variant(variant: int) -> None:
+    """Kernel variant of later nvfp4_gemm_epilogue / nvfp4_grouped_gemm calls (-1 = automatic)."""
+    check(lib().b2_nvfp4_grouped_gemm_set_variant(int(variant)), "b2_nvfp4_grouped_gemm_set_variant")
+
+
+def nvfp4_grouped_gemm_status() -> None:
+    check(lib().b2_nvfp4_grouped_gemm_status(current_stream_ptr()), "b2_nvfp4_grouped_gemm_status")
+
+
+def nvfp4_quantize_grouped(inp, index, offsets, out, sf, global_scale, in_rows: int, rows: int, groups: int, k: int,
+                           dtype: str, fuse_silu: bool = False) -> None:
+    """Quantizes row index[r] of `inp` into row r (row r without index), scales in the grouped 128x4 layout."""
+    _require_here(inp, index, offsets, out, sf, global_scale)
+    check(
+        lib().b2_nvfp4_quantize_grouped(_ptr(inp), _ptr_or_null(index), _ptr(offsets), _ptr(out), _ptr(sf),
+                                        _ptr(global_scale), in_rows, rows, groups, k, DTYPE_CODES[dtype],
+                                        int(fuse_silu), current_stream_ptr()),
+        "b2_nvfp4_quantize_grouped",
+    )
+
+
+def moe_plan(ids, offsets, row_token, position, tokens: int, topk: int, experts: int) -> None:
+    _require_here(ids, offsets, row_token, position)
+    check(
+        lib().b2_moe_plan(_ptr(ids), _ptr(offsets), _ptr(row_token), _ptr(position), tokens, topk, experts,
+                          current_stream_ptr()),
+        "b2_moe_plan",
+    )
+
+
+def moe_combine(y, position, weight, residual, out, rows: int, tokens: int, topk: int, n: int, dtype: str) -> None:
+    """out[t] = residual[t] + sum_k weight[t, k] * y[position[t, k]]; residual may be None."""
+    _require_here(y, position, weight, residual, out)
+    check(
+        lib().b2_moe_combine(_ptr(y), _ptr(position), _ptr(weight), _ptr_or_null(residual), _ptr(out), rows, tokens,
+                             topk, n, DTYPE_CODES[dtype], current_stream_ptr()),
+        "b2_moe_combine",
+    )
+
+
+def moe_expert_ffn(x, ids, weight, w1, sf1, alpha1, gs1, w2, sf2, alpha2, gs2, residual, out, workspace, tokens: int,
+                   topk: int, experts: int, hidden: int, inner: int, dtype: str) -> None:
+    _require_here(x, ids, weight, w1, sf1, alpha1, gs1, w2, sf2, alpha2, gs2, residual, out, workspace)
+    check(
+        lib().b2_moe_expert_ffn(_ptr(x), _ptr(ids), _ptr(weight), _ptr(w1), _ptr(sf1), _ptr(alpha1), _ptr(gs1),
+                                _ptr(w2), _ptr(sf2), _ptr(alpha2), _ptr(gs2), _ptr_or_null(residual), _ptr(out),
+                                _ptr(workspace), workspace.numel(), tokens, topk, experts, hidden, inner,
+                                DTYPE_CODES[dtype], current_stream_ptr()),
+        "b2_moe_expert_ffn",
+    )
+
+
+def gated_add_rmsnorm_fp4quant(x, residual, w_post, gate, w_pre, residual_out, y, sf, global_scale, M: int, H: int,
+                               rows_per_gate: int, residual_scale: float, eps: float, dtype: str, quantize: bool,
+                               swizzled: bool) -> None:
+    """w_post and gate may be None; sf and global_scale are None without `quantize`."""
+    _require_here(x, residual, w_post, gate, w_pre, residual_out, y, sf, global_scale)
+    check(
+        lib().b2_gated_add_rmsnorm_fp4quant(_ptr(x), _ptr(residual), _ptr_or_null(w_post), _ptr_or_null(gate),
+                                            _ptr(w_pre), _ptr(residual_out), _ptr(y), _ptr_or_null(sf),
+                                            _ptr_or_null(global_scale), M, H, rows_per_gate, float(residual_scale),
+                                            float(eps), DTYPE_CODES[dtype], int(quantize), int(swizzled),
+                                            current_stream_ptr()),
+        "b2_gated_add_rmsnorm_fp4quant",
     )
 
 

@@ -22,9 +22,11 @@ def bench_configs(module) -> list:
 
 
 def find_bench_config(module, label: str) -> dict:
+    from tirx_kernels.registry import module_meta
+
     matches = [c for c in bench_configs(module) if c.get("label") == label]
     if len(matches) != 1:
-        raise KeyError(f"kernel {module.KERNEL_META['name']!r} config {label!r}: "
+        raise KeyError(f"kernel {module_meta(module)['name']!r} config {label!r}: "
                        f"expected exactly one match, found {len(matches)}")
     return matches[0]
 
@@ -66,7 +68,7 @@ def main() -> None:
     if args.json or args.json_file:
         os.environ["TIRX_BENCH_JSON"] = "1"
 
-    from tirx_kernels.registry import discover_kernels, load_kernel
+    from tirx_kernels.registry import discover_kernels, load_kernel, module_meta
     from tirx_kernels.runner import (DEFAULT_BENCH_COOLDOWN_S, DEFAULT_BENCH_ROUNDS, run_kernel_bench,
                                      set_external_references_enabled)
 
@@ -86,9 +88,9 @@ def main() -> None:
         except KeyError:
             print(f"ERROR: kernel '{args.kernel}' not found.", file=sys.stderr)
             sys.exit(1)
-        if args.cc is not None and module.KERNEL_META.get("compute_capability") != args.cc:
+        if args.cc is not None and module_meta(module).get("compute_capability") != args.cc:
             print(f"ERROR: kernel '{args.kernel}' compute_capability="
-                  f"{module.KERNEL_META.get('compute_capability')} != filter {args.cc}", file=sys.stderr)
+                  f"{module_meta(module).get('compute_capability')} != filter {args.cc}", file=sys.stderr)
             sys.exit(1)
         kernels = {args.kernel: module}
     else:

@@ -26,6 +26,10 @@ NON_CATEGORY_DIRS = frozenset({"bench", "test", "bench_suite", "experimental"})
 HELPER_SUBPACKAGES = frozenset({"utils"})
 _META_FIELDS = (("name", str), ("category", str), ("compute_capability", int))
 _ASSIGN_RE = re.compile(r"^KERNEL_META\s*=", re.MULTILINE)
+# Operators of this package that the reference's registry does not have declare OPERATOR_META, with the fields of
+# KERNEL_META.  They are looked up by name (load_kernel, both CLIs' --kernel) and listed by operator_index; the
+# drop-in kernel list stays the reference's.
+_FIELDS = ("KERNEL_META", "OPERATOR_META")
 
 
 @dataclass(frozen=True)
@@ -77,10 +81,11 @@ def _meta_problems(meta, category: str) -> list[str]:
     return problems
 
 
-def _read_literal_meta(path: Path) -> dict | None:
-    """The dict literal assigned to a module-level ``KERNEL_META``, or None when absent."""
+def _read_literal_meta(path: Path, field: str = "KERNEL_META") -> dict | None:
+    """The dict literal assigned to a module-level ``KERNEL_META`` (or `field`), or None when absent."""
     text = path.read_text(encoding="utf-8")
-    if not _ASSIGN_RE.search(text):
+    pattern = _ASSIGN_RE if field == "KERNEL_META" else re.compile(rf"^{field}\s*=", re.MULTILINE)
+    if not pattern.search(text):
         return None
     found = []
     for node in ast.parse(text, filename=str(path)).body:
@@ -89,17 +94,17 @@ def _read_literal_meta(path: Path) -> dict | None:
             targets = node.targets
         elif isinstance(node, ast.AnnAssign) and node.value is not None:
             targets = [node.target]
-        if any(isinstance(t, ast.Name) and t.id == "KERNEL_META" for t in targets):
+        if any(isinstance(t, ast.Name) and t.id == field for t in targets):
             value = ast.literal_eval(node.value)
             if not isinstance(value, dict):
-                raise ValueError(f"{path} KERNEL_META must be a literal dict")
+                raise ValueError(f"{path} {field} must be a literal dict")
             found.append(value)
     if len(found) > 1:
-        raise ValueError(f"{path} assigns KERNEL_META more than once")
+        raise ValueError(f"{path} assigns {field} more than once")
     return found[0] if found else None
 
 
-_INDEX_CACHE: dict = {"stamp": None, "records": {}, "diagnostics": ()}
+_INDEX_CACHE: dict = {field: {"stamp": None, "records": {}, "diagnostics": ()} for field in _FIELDS}
 
 
 def _scan() -> tuple[tuple, list[tuple[str, str, Path]]]:
@@ -113,24 +118,24 @@ def _scan() -> tuple[tuple, list[tuple[str, str, Path]]]:
     return tuple(stamp), candidates
 
 
-def kernel_index(*, strict: bool = False) -> dict[str, KernelRecord]:
-    """Public name -> record, rebuilt only when a candidate source file changes."""
+def _index(field: str, strict: bool) -> dict[str, KernelRecord]:
     stamp, candidates = _scan()
-    if _INDEX_CACHE["stamp"] != stamp:
+    cache = _INDEX_CACHE[field]
+    if cache["stamp"] != stamp:
         records: dict[str, KernelRecord] = {}
         diagnostics = []
         for category, relative, path in candidates:
             module_name = f"tirx_kernels.{category}.{relative}"
             try:
-                meta = _read_literal_meta(path)
+                meta = _read_literal_meta(path, field)
             except (SyntaxError, ValueError) as error:
-                diagnostics.append(f"{path} has invalid KERNEL_META: {error}")
+                diagnostics.append(f"{path} has invalid {field}: {error}")
                 continue
             if meta is None:
                 continue
             problems = _meta_problems(meta, category)
             if problems:
-                diagnostics.append(f"{module_name} has invalid KERNEL_META: " + "; ".join(problems))
+                diagnostics.append(f"{module_name} has invalid {field}: " + "; ".join(problems))
                 continue
             if meta["name"] in records:
                 raise ValueError(
@@ -139,16 +144,31 @@ def kernel_index(*, strict: bool = False) -> dict[str, KernelRecord]:
                 )
             records[meta["name"]] = KernelRecord(meta["name"], category, meta["compute_capability"],
                                                  module_name, path)
-        _INDEX_CACHE.update(stamp=stamp, records=records, diagnostics=tuple(diagnostics))
-    if _INDEX_CACHE["diagnostics"]:
+        cache.update(stamp=stamp, records=records, diagnostics=tuple(diagnostics))
+    if cache["diagnostics"]:
         if strict:
-            raise ValueError(_INDEX_CACHE["diagnostics"][0])
-        for message in _INDEX_CACHE["diagnostics"]:
+            raise ValueError(cache["diagnostics"][0])
+        for message in cache["diagnostics"]:
             _log.warning(message)
-    return dict(_INDEX_CACHE["records"])
+    return dict(cache["records"])
 
 
-def _import_checked(record: KernelRecord, *, strict: bool) -> ModuleType | None:
+def kernel_index(*, strict: bool = False) -> dict[str, KernelRecord]:
+    """Public name -> record, rebuilt only when a candidate source file changes."""
+    return _index("KERNEL_META", strict)
+
+
+def operator_index(*, strict: bool = False) -> dict[str, KernelRecord]:
+    """The same for the operators beyond the reference's registry (``OPERATOR_META``)."""
+    return _index("OPERATOR_META", strict)
+
+
+def module_meta(module: ModuleType) -> dict:
+    """``KERNEL_META`` of a kernel module, ``OPERATOR_META`` of an operator module."""
+    return getattr(module, "KERNEL_META", None) or module.OPERATOR_META
+
+
+def _import_checked(record: KernelRecord, *, strict: bool, field: str = "KERNEL_META") -> ModuleType | None:
     try:
         module = importlib.import_module(record.module_name)
     except Exception as error:
@@ -156,7 +176,7 @@ def _import_checked(record: KernelRecord, *, strict: bool) -> ModuleType | None:
             raise
         _log.warning("tirx_kernels: failed to import %s: %s", record.module_name, error)
         return None
-    meta = getattr(module, "KERNEL_META", None)
+    meta = getattr(module, field, None)
     problems = _meta_problems(meta, record.category)
     if isinstance(meta, dict):
         if meta.get("name") != record.name:
@@ -164,7 +184,7 @@ def _import_checked(record: KernelRecord, *, strict: bool) -> ModuleType | None:
         if meta.get("compute_capability") != record.compute_capability:
             problems.append("runtime compute_capability does not match source index")
     if problems:
-        message = f"{record.module_name} has invalid runtime KERNEL_META: " + "; ".join(problems)
+        message = f"{record.module_name} has invalid runtime {field}: " + "; ".join(problems)
         if strict:
             raise ValueError(message)
         _log.warning(message)
@@ -173,9 +193,14 @@ def _import_checked(record: KernelRecord, *, strict: bool) -> ModuleType | None:
 
 
 def load_kernel(name: str, *, strict: bool = False) -> ModuleType:
-    """Import the one module whose ``KERNEL_META['name']`` is `name`; KeyError if there is none."""
+    """Import the one module whose ``KERNEL_META['name']`` (or else ``OPERATOR_META['name']``) is `name`; KeyError if
+    there is none."""
+    field = "KERNEL_META"
     record = kernel_index(strict=strict).get(name)
-    module = _import_checked(record, strict=strict) if record is not None else None
+    if record is None:
+        field = "OPERATOR_META"
+        record = operator_index(strict=strict).get(name)
+    module = _import_checked(record, strict=strict, field=field) if record is not None else None
     if module is None:
         raise KeyError(name)
     return module

@@ -11,7 +11,7 @@ import sys
 import traceback
 from unittest import SkipTest
 
-from tirx_kernels.registry import discover_kernels
+from tirx_kernels.registry import discover_kernels, load_kernel, module_meta, operator_index
 from tirx_kernels.runner import run_kernel_test
 
 
@@ -52,6 +52,10 @@ def main() -> None:
 
     kernels = discover_kernels(min_compute_capability=args.cc)
     if args.kernel:
+        if args.kernel not in kernels and args.kernel in operator_index():  # not one of the reference's kernels
+            module = load_kernel(args.kernel)
+            if args.cc is None or module_meta(module)["compute_capability"] == args.cc:
+                kernels[args.kernel] = module
         if args.kernel not in kernels:
             print(f"ERROR: kernel '{args.kernel}' not found. Available: {sorted(kernels)}")
             sys.exit(1)
