@@ -22,10 +22,10 @@
 //     multiplied (zeros, or the next group's weights) and dropped;
 //   * 32-row tiles for groups of a few rows (AM = 32) may start in any quarter of a 128-row scale tile; the scale
 //     warps move that quarter to the first place;
-//   * with NACC == 2 the accumulator is double: the next tile is multiplied while the epilogue works.
-//
-// The residual is loaded into the registers that later hold the packed output, before the wait for the
-// accumulator: its latency hides behind the products and costs no register.
+//   * the epilogue takes its part of the accumulator into registers as raw fp32 and hands tensor memory back before it
+//     computes anything: bias, activation, residual and stores run beside the next tile's products.  The 256 x 256 pair
+//     has 16 epilogue warps for that (64 columns of fp32 a thread; 8 warps would need 128) and moves registers to them
+//     with setmaxnreg; with NACC == 2 the accumulator itself is double.
 #include <atomic>
 
 #include "nvfp4_tile.cuh"
@@ -33,10 +33,9 @@
 namespace b2 {
 namespace {
 
-constexpr int kGroupThreads = 640;  // 4 issuing warps, 2 x 4 scale warps, 8 epilogue warps
 constexpr int kMaxGroups = 384;     // bounds the tables in shared memory
 constexpr int kTableBytes = 2 * (kMaxGroups + 1) * 4;
-constexpr int kGWarpOperands = 0, kGWarpMma = 1, kGWarpScales = 2, kGWarpMma2 = 3, kGWarpScale0 = 4, kGWarpEpi0 = 12;
+constexpr int kGWarpOperands = 0, kGWarpMma = 1, kGWarpScales = 2, kGWarpMma2 = 3, kGWarpScale0 = 4;
 
 struct GroupedParams {
   const float* alpha;       // [groups]
@@ -47,6 +46,7 @@ struct GroupedParams {
   uint32_t* status;
   int rows, groups, N;
   int k_slabs;
+  int tiles_m;              // row tiles of the single group when there are no offsets
   int tiles_n, group_n;
   int act;                  // B2_ACT_*
   int fp16;                 // 16-bit type of bias, residual and D
@@ -69,6 +69,14 @@ struct Tile {
 // Work item t -> its tile.  starts[g] is the number of row tiles in front of group g; among groups without rows,
 // which share a start, bisection ends at the last one, the one that has the tile.
 __device__ __forceinline__ Tile find_tile(const GroupedParams& p, const int* starts, const int* rows, int t) {
+  Tile r;
+  if (!p.offsets) {
+    r.group = 0;
+    r.first = 0;
+    r.last = p.rows;
+    tile_coords(t, p.tiles_m, p.tiles_n, p.group_n, r.tm, r.tn);
+    return r;
+  }
   const int q = t / p.tiles_n;
   int lo = 0, hi = p.groups;
   while (hi - lo > 1) {
@@ -76,7 +84,6 @@ __device__ __forceinline__ Tile find_tile(const GroupedParams& p, const int* sta
     if (starts[mid] <= q) lo = mid;
     else hi = mid;
   }
-  Tile r;
   r.group = lo;
   r.first = rows[lo];
   r.last = rows[lo + 1];
@@ -105,15 +112,6 @@ __device__ __forceinline__ float gelu_erf(float v) {
   return v * (v >= 0.0f ? 1.0f - half_tail : half_tail);
 }
 
-__device__ __forceinline__ float2 unpack_pair(uint32_t w, bool fp16) {
-  const float2 h = unpack2<F16Tag>(w), b = unpack2<BF16Tag>(w);
-  return make_float2(fp16 ? h.x : b.x, fp16 ? h.y : b.y);
-}
-__device__ __forceinline__ uint32_t pack_pair(float x, float y, bool fp16) {
-  const uint32_t h = pack_from_f32<F16Tag>(x, y), b = pack_from_f32<BF16Tag>(x, y);
-  return fp16 ? h : b;
-}
-
 // Not the read-only path: the residual may be the output's own memory (every word is read before it is written, by
 // the thread that writes it).
 __device__ __forceinline__ uint4 load_residual(const uint16_t* p) {
@@ -121,58 +119,82 @@ __device__ __forceinline__ uint4 load_residual(const uint16_t* p) {
   asm volatile("ld.global.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
   return r;
 }
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
-// 32 accumulator columns of one row -> 16 packed words.  `io` holds the residual on entry.
-__device__ __forceinline__ void finish32(const GroupedParams& p, uint32_t (&v)[32], uint32_t* io, const uint16_t* bias,
-                                         int col, float alpha) {
-  const bool fp16 = p.fp16 != 0;
-  float f[32];
+// 8 accumulator columns of one row -> 4 packed words of the output.  `bias` is null or points at the first of the
+// columns, `add` says whether `r` is a part of the residual.  Eight at a time: the raw accumulator takes up to 64
+// registers, little else may live beside it.
+template <typename Tag>
+__device__ __forceinline__ void finish8(int act, float alpha, const uint16_t* bias, bool add, uint4 r, const uint32_t* v,
+                                        uint32_t* out) {
+  float f[8];
 #pragma unroll
-  for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(v[i]) * alpha;
+  for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(v[i]) * alpha;
   if (bias) {
+    const uint4 b = __ldg(reinterpret_cast<const uint4*>(bias));
+    const uint32_t w[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      if (col + 8 * c < p.N) {  // N is a multiple of 8
-        const uint4 b = __ldg(reinterpret_cast<const uint4*>(bias + col + 8 * c));
-        const uint32_t w[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 x = unpack_pair(w[i], fp16);
-          f[8 * c + 2 * i] += x.x;
-          f[8 * c + 2 * i + 1] += x.y;
-        }
-      }
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] += unpack_lo<Tag>(w[i]);
+      f[2 * i + 1] += unpack_hi<Tag>(w[i]);
     }
   }
-  if (p.act == B2_ACT_SILU || p.act == B2_ACT_GELU_TANH) {
-    const float c1 = p.act == B2_ACT_SILU ? 1.4426950408889634f : 2.3022081983375f;
-    const float c2 = p.act == B2_ACT_SILU ? 0.0f : 0.10294324f;
+  if (act == B2_ACT_SILU || act == B2_ACT_GELU_TANH) {
+    const float c1 = act == B2_ACT_SILU ? 1.4426950408889634f : 2.3022081983375f;
+    const float c2 = act == B2_ACT_SILU ? 0.0f : 0.10294324f;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) f[i] = gate_sigmoid(f[i], c1, c2);
-  } else if (p.act == B2_ACT_GELU) {
+    for (int i = 0; i < 8; ++i) f[i] = gate_sigmoid(f[i], c1, c2);
+  } else if (act == B2_ACT_GELU) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) f[i] = gelu_erf(f[i]);
-  } else if (p.act == B2_ACT_RELU) {
+    for (int i = 0; i < 8; ++i) f[i] = gelu_erf(f[i]);
+  } else if (act == B2_ACT_RELU) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) f[i] = f[i] < 0.0f ? 0.0f : f[i];  // a NaN stays one
+    for (int i = 0; i < 8; ++i) f[i] = f[i] < 0.0f ? 0.0f : f[i];  // a NaN stays one
   }
-  if (p.residual) {
+  if (add) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float2 r = unpack_pair(io[i], fp16);
-      f[2 * i] += r.x;
-      f[2 * i + 1] += r.y;
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] += unpack_lo<Tag>(w[i]);
+      f[2 * i + 1] += unpack_hi<Tag>(w[i]);
     }
   }
 #pragma unroll
-  for (int i = 0; i < 16; ++i) io[i] = pack_pair(f[2 * i], f[2 * i + 1], fp16);
+  for (int i = 0; i < 4; ++i) out[i] = pack_from_f32<Tag>(f[2 * i], f[2 * i + 1]);
+}
+
+__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+template <int N>
+__device__ __forceinline__ void bulk_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+template <int REGS>
+__device__ __forceinline__ void give_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS));
+}
+template <int REGS>
+__device__ __forceinline__ void take_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS));
 }
 
 // CG: CTAs of a tile (1 or 2).  BN: its columns.  AM: rows of A that one CTA loads and multiplies (the MMA reads 128;
 // what follows a shorter box in the stage only reaches accumulator rows that nobody reads).  MMAS: MMA-issuing warps
 // with an accumulator each, for a single tile per CTA (issuing is the limit there).  NACC: accumulators in turn, for many tiles.
-template <int CG, int BN, int STAGES, int TMA_OUT, int AM, int MMAS, int NACC>
-__global__ void __launch_bounds__(kGroupThreads, 1)
+// SETS of 4 scale warps and PARTS of 4 epilogue warps, each with BN / PARTS columns.
+constexpr int group_threads(int sets, int parts) { return 32 * (4 + 4 * sets + 4 * parts); }
+// Registers a thread of each warpgroup has when PARTS == 4 (768 threads start with 80 each): 6 x 80 = 56 + 40 + 4 x 96.
+constexpr int kRegsLaunch = 80, kRegsIssue = 56, kRegsScale = 40, kRegsEpilogue = 96;
+static_assert(kRegsIssue + kRegsScale + 4 * kRegsEpilogue <= 6 * kRegsLaunch, "no warpgroup waits for registers that nobody gives");
+
+template <int CG, int BN, int STAGES, int TMA_OUT, int AM, int MMAS, int NACC, int SETS, int PARTS>
+__global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
     nvfp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                               const __grid_constant__ CUtensorMap map_sfa, const __grid_constant__ CUtensorMap map_sfb,
                               const __grid_constant__ CUtensorMap map_d, const __grid_constant__ GroupedParams p) {
@@ -187,6 +209,10 @@ __global__ void __launch_bounds__(kGroupThreads, 1)
   constexpr uint32_t kOperandTx = static_cast<uint32_t>(L::kABytes + L::kBBytes) * CG;
   constexpr uint32_t kScaleTx = static_cast<uint32_t>(L::kSfaBytes + L::kSfbBytes);
   constexpr bool kWarpWide = CG == 2;  // issuing roles run as whole warps (see nvfp4_gemm.cu)
+  constexpr int kCols = BN / PARTS;    // columns of an epilogue warp
+  constexpr int kWarpEpi0 = kGWarpScale0 + 4 * SETS;
+  constexpr bool kMoveRegisters = PARTS == 4;
+  static_assert((kCols == 32 || kCols == 64) && (!kMoveRegisters || SETS == 1), "epilogue shapes");
 
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -222,7 +248,7 @@ __global__ void __launch_bounds__(kGroupThreads, 1)
     }
     for (int a = 0; a < NACC; ++a) {
       mbar_init(acc_full_bar(a), MMAS);
-      mbar_init(acc_empty_bar(a), 8 * CG);  // one arrive per epilogue warp of every CTA in the group
+      mbar_init(acc_empty_bar(a), 4 * PARTS * CG);  // one arrive per epilogue warp of every CTA in the group
     }
     *abort_flag = 0u;
     fence_barrier_init();
@@ -237,19 +263,15 @@ __global__ void __launch_bounds__(kGroupThreads, 1)
   }
   // Dependent launch as in nvfp4_gemm.cu: nothing in front of this wait touches global memory.
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (warp == kGWarpMma2) {
+  if (p.offsets && warp == kGWarpMma2) {
     int tiles = 0;  // row tiles in front of the 32 groups of this step
     for (int g0 = 0; g0 < p.groups; g0 += 32) {
       const int g = g0 + lane;
       int first = 0, last = 0;
       if (g < p.groups) {
         // Offsets that are not ascending or leave [0, rows] are brought back into it: no access leaves A or D.
-        if (p.offsets) {
-          first = min(max(__ldg(p.offsets + g), 0), p.rows);
-          last = min(max(__ldg(p.offsets + g + 1), first), p.rows);
-        } else {
-          last = p.rows;
-        }
+        first = min(max(__ldg(p.offsets + g), 0), p.rows);
+        last = min(max(__ldg(p.offsets + g + 1), first), p.rows);
       }
       const int mine = (last - first + kBM - 1) / kBM;
       int sum = mine;
@@ -275,7 +297,10 @@ __global__ void __launch_bounds__(kGroupThreads, 1)
   tc_fence_after();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t tmem_base = kWarpWide ? __shfl_sync(0xffffffffu, *tmem_slot, 0) : *tmem_slot;
-  const int num_tiles = starts[p.groups] * p.tiles_n;
+  // What the issuing warps compute from shared memory is made uniform by a shuffle, or the compiler would keep their
+  // loops' state out of uniform registers (nvfp4_gemm.cu).
+  auto uniform = [](int v) { return kWarpWide ? __shfl_sync(0xffffffffu, v, 0) : v; };
+  const int num_tiles = p.offsets ? uniform(starts[p.groups]) * p.tiles_n : p.tiles_m * p.tiles_n;
   const int k_slabs = p.k_slabs;
 
   // The waits of the issuing roles: of the whole warp with one outcome, or of lane 0.
@@ -286,6 +311,10 @@ __global__ void __launch_bounds__(kGroupThreads, 1)
   };
   auto issues = [&] { return kWarpWide ? elect_one() : true; };
 
+  // setmaxnreg stands in front of the roles of its warpgroup, inside one branch: behind a point where branches with
+  // different limits meet, the compiler keeps to the lowest.
+  if (warp < kGWarpScale0) {
+  if constexpr (kMoveRegisters) give_registers<kRegsIssue>();
   if (warp == kGWarpOperands) {
     // ================= TMA producer of the operands =================
     if (kWarpWide || lane == 0) {
@@ -294,8 +323,8 @@ __global__ void __launch_bounds__(kGroupThreads, 1)
       bool alive = true;
       for (int t = unit; t < num_tiles && alive; t += num_units) {
         const Tile tile = find_tile(p, starts, group_rows, t);
-        const int row_a = tile.first + tile.tm * kBM + static_cast<int>(rank) * kBlockM;
-        const int row_b = tile.group * p.N + tile.tn * BN + static_cast<int>(rank) * L::kBRows;
+        const int row_a = uniform(tile.first + tile.tm * kBM) + static_cast<int>(rank) * kBlockM;
+        const int row_b = uniform(tile.group * p.N + tile.tn * BN) + static_cast<int>(rank) * L::kBRows;
         for (int ks = 0; ks < k_slabs; ++ks) {
           if (!role_wait(empty_bar(stage), phase ^ 1u, 1u)) { alive = false; break; }
           const uint32_t sbase = smem_base + stage * L::kStageBytes;
@@ -320,8 +349,8 @@ __global__ void __launch_bounds__(kGroupThreads, 1)
       bool alive = true;
       for (int t = unit; t < num_tiles && alive; t += num_units) {
         const Tile tile = find_tile(p, starts, group_rows, t);
-        const int sfa_tile = (tile.first >> 7) + tile.group + ((tile.tm * kBM) >> 7) + static_cast<int>(rank);
-        const int sfb_tile = tile.group * sfb_tiles + (tile.tn * BN) / 128;
+        const int sfa_tile = uniform((tile.first >> 7) + tile.group + ((tile.tm * kBM) >> 7)) + static_cast<int>(rank);
+        const int sfb_tile = uniform(tile.group * sfb_tiles + (tile.tn * BN) / 128);
         for (int ks = 0; ks < k_slabs; ++ks) {
           if (!role_wait(empty_bar(stage), phase ^ 1u, 1u)) { alive = false; break; }
           const uint32_t sf_smem = smem_base + stage * L::kStageBytes + L::kABytes + L::kBBytes;
@@ -392,9 +421,12 @@ __global__ void __launch_bounds__(kGroupThreads, 1)
         if (++acc == NACC) { acc = 0; acc_phase ^= 1u; }
       }
     }
-  } else if (warp >= kGWarpScale0 && warp < kGWarpEpi0) {
+  }
+  } else if (warp < kWarpEpi0) {
+    if constexpr (kMoveRegisters) give_registers<kRegsScale>();
     // ================= scale warps: shared memory -> registers -> tensor memory =================
-    // Layout and reasons as in nvfp4_gemm.cu.  Two sets of four warps, by the parity of the stage.
+    // Layout and reasons as in nvfp4_gemm.cu.  Two sets of four warps share the stages by parity; one set is enough
+    // where a slab's products take longer (256 columns: 520 cycles) than the way of its scales (about 250).
     const int quarter = warp & 3;
     const int set = (warp - kGWarpScale0) >> 2;
     const int total_slabs = unit < num_tiles ? ((num_tiles - unit + num_units - 1) / num_units) * k_slabs : 0;
@@ -410,18 +442,16 @@ __global__ void __launch_bounds__(kGroupThreads, 1)
         --tile_slabs;
       }
       const int stage = n % STAGES;
-      if ((stage & 1) != set) continue;
+      if (SETS == 2 && (stage & 1) != set) continue;
       const uint32_t phase = static_cast<uint32_t>(n / STAGES) & 1u;
       if (!wait_or_abort(sfload_bar(stage), phase, ctx, 5u)) break;
       const uint32_t sfa_smem = smem_base + stage * L::kStageBytes + L::kABytes + L::kBBytes + lane * 16;
       const uint32_t sfb_smem = sfa_smem + L::kSfaBytes;
-      uint32_t a[16], b[16 * L::kChunks];
+      const uint32_t dst = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + kAccCols + stage * L::kSfCols;
+      // Sixteen words at a time: with a slab's 48 in flight the warp would need registers that the epilogue wants.
+      uint32_t a[16];
 #pragma unroll
       for (int kb = 0; kb < 4; ++kb) lds128(sfa_smem + kb * 512, a + 4 * kb);
-#pragma unroll
-      for (int kb = 0; kb < 4; ++kb)
-#pragma unroll
-        for (int c = 0; c < L::kChunks; ++c) lds128(sfb_smem + (c * 4 + kb) * 512, b + 4 * (kb * L::kChunks + c));
       if constexpr (AM == 32) {
 #pragma unroll
         for (int kb = 0; kb < 4; ++kb) {
@@ -429,10 +459,17 @@ __global__ void __launch_bounds__(kGroupThreads, 1)
           a[4 * kb] = part & 2 ? high : low;
         }
       }
-      const uint32_t dst = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + kAccCols + stage * L::kSfCols;
       tmem_st_32x32_x16(dst, a);
 #pragma unroll
-      for (int c = 0; c < L::kChunks; ++c) tmem_st_32x32_x16(dst + 16 + 16 * c, b + 16 * c);
+      for (int c = 0; c < L::kChunks; ++c) {  // words 16 c .. 16 c + 15 of [kb][chunk][4]
+        uint32_t b[16];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int word = 4 * c + i;
+          lds128(sfb_smem + ((word % L::kChunks) * 4 + word / L::kChunks) * 512, b + 4 * i);
+        }
+        tmem_st_32x32_x16(dst + 16 + 16 * c, b);
+      }
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -441,13 +478,19 @@ __global__ void __launch_bounds__(kGroupThreads, 1)
         else mbar_arrive_cluster_relaxed(mapa_shared(full_bar(stage), 0));
       }
     }
-  } else if (warp >= kGWarpEpi0) {
-    // ================= epilogue: 8 warps, lane quarter = warp & 3, column half = (warp - 12) / 4 ===========
-    constexpr int kHalf = BN / 2;
+  } else {
+    if constexpr (kMoveRegisters) take_registers<kRegsEpilogue>();
+    // ================= epilogue: lane quarter = warp & 3, column part = (warp - first) / 4 ===========
     const int quarter = warp & 3;
-    const int half = (warp - kGWarpEpi0) >> 2;
+    const int part = (warp - kWarpEpi0) >> 2;
     const uint64_t store_policy = l2_policy_evict_first();
     const bool two = MMAS == 2 && k_slabs > 1;  // a single slab leaves the second issuer without one
+    // Staging of the TMA store: buffers of 16 rows x 64 columns per warp, 128-byte rows, 128-byte swizzle.  (Boxes of
+    // 32 x 32, with 64-byte rows, take the TMA twice as long: 16384 rows of 32 groups, N = 2048, K = 1408: 98 us for 49.)
+    static_assert(TMA_OUT == 0 || kCols == 64, "store boxes");
+    constexpr int kBufs = TMA_OUT > 0 ? L::kStagingBytes / (4 * PARTS * 2048) : 1;
+    static_assert(kBufs == 1 || kBufs == 2, "store buffers");
+    const uint32_t staging = smem_base + STAGES * L::kStageBytes + static_cast<uint32_t>(warp - kWarpEpi0) * kBufs * 2048u;
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int t = unit; t < num_tiles; t += num_units) {
@@ -456,43 +499,34 @@ __global__ void __launch_bounds__(kGroupThreads, 1)
       const int in_tile = static_cast<int>(rank) * kBlockM + quarter * 32;  // first row of this warp in the tile
       const int row0 = tile.first + tile.tm * kBM + in_tile;
       const int row = row0 + lane;
-      const int col0 = tile.tn * BN + half * kHalf;
+      const int col0 = tile.tn * BN + part * kCols;
       const bool any = in_tile < kBM && row0 < tile.last && col0 < p.N;  // the same in the whole warp
       const bool mine = any && row < tile.last;
       const int64_t at = static_cast<int64_t>(row) * p.N + col0;
-      const uint16_t* bias = p.bias ? p.bias + static_cast<int64_t>(tile.group) * p.N : nullptr;
-      uint32_t packed[kHalf / 2];
-      if (p.residual) {
-#pragma unroll
-        for (int i = 0; i < kHalf / 8; ++i) {
-          uint4 r = make_uint4(0u, 0u, 0u, 0u);
-          if (mine && col0 + 8 * i < p.N) r = load_residual(p.residual + at + 8 * i);
-          packed[4 * i] = r.x;
-          packed[4 * i + 1] = r.y;
-          packed[4 * i + 2] = r.z;
-          packed[4 * i + 3] = r.w;
-        }
-      }
+      const uint16_t* bias = p.bias ? p.bias + static_cast<int64_t>(tile.group) * p.N + col0 : nullptr;
+      const uint16_t* residual = p.residual && mine ? p.residual + at : nullptr;
+      if (residual) prefetch_l2(residual);
       if (!wait_or_abort(acc_full_bar(acc), acc_phase, ctx, 4u)) break;
       tc_fence_after();
+      uint32_t v[kCols];
       if (any) {
         const uint32_t acc_tmem = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
-                                  static_cast<uint32_t>(acc * MMAS * BN + half * kHalf);
+                                  static_cast<uint32_t>(acc * MMAS * BN + part * kCols);
 #pragma unroll
-        for (int c0 = 0; c0 < kHalf; c0 += 32) {
-          uint32_t v[32];
-          tmem_ld_32x32(acc_tmem + c0, v);
-          if constexpr (MMAS == 2) {
-            if (two) {
-              uint32_t v2[32];
-              tmem_ld_32x32(acc_tmem + BN + c0, v2);
+        for (int c0 = 0; c0 < kCols; c0 += 32)
+          tmem_ld_32x32(acc_tmem + c0, *reinterpret_cast<uint32_t(*)[32]>(v + c0));
+        tmem_ld_wait();
+        if constexpr (MMAS == 2) {
+          if (two) {
+#pragma unroll
+            for (int c0 = 0; c0 < kCols; c0 += 16) {
+              uint32_t w[16];
+              tmem_ld_32x16(acc_tmem + BN + c0, w);
               tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) + __uint_as_float(v2[i]));
+              for (int i = 0; i < 16; ++i) v[c0 + i] = __float_as_uint(__uint_as_float(v[c0 + i]) + __uint_as_float(w[i]));
             }
           }
-          tmem_ld_wait();
-          finish32(p, v, packed + c0 / 2, bias, col0 + c0, alpha);
         }
       }
       tc_fence_before();
@@ -504,28 +538,35 @@ __global__ void __launch_bounds__(kGroupThreads, 1)
       if (++acc == NACC) { acc = 0; acc_phase ^= 1u; }
       if (!any) continue;
       // The TMA clips rows behind the last row and columns behind N, but knows nothing of groups.
-      if (TMA_OUT > 0 && (row0 + 32 <= tile.last || tile.last == p.rows)) {
+      const bool by_tma = TMA_OUT > 0 && (row0 + 32 <= tile.last || tile.last == p.rows);
+      uint32_t* const out = v;  // packed words take the place of accumulators that are done
+      uint4 next = make_uint4(0u, 0u, 0u, 0u);  // the residual's part of the next eight columns, on its way
+      if (residual) next = load_residual(residual);
+#pragma unroll
+      for (int c0 = 0; c0 < kCols; c0 += 8) {
+        const uint4 r = next;
+        if (residual && c0 + 8 < kCols && col0 + c0 + 8 < p.N) next = load_residual(residual + c0 + 8);
+        const uint16_t* b = bias && col0 + c0 < p.N ? bias + c0 : nullptr;
+        if (p.fp16) finish8<F16Tag>(p.act, alpha, b, residual != nullptr, r, v + c0, out + c0 / 2);
+        else finish8<BF16Tag>(p.act, alpha, b, residual != nullptr, r, v + c0, out + c0 / 2);
+      }
+      if (TMA_OUT > 0 && by_tma) {
         if constexpr (TMA_OUT > 0) {
-          constexpr int kSubs = kHalf / 64;
-          const uint32_t staging = smem_base + STAGES * L::kStageBytes +
-                                   static_cast<uint32_t>(warp - kGWarpEpi0) * TMA_OUT * 4096u;
 #pragma unroll
-          for (int sub = 0; sub < kSubs; ++sub) {
-            if (sub % TMA_OUT == 0) {
-              if (lane == 0) bulk_wait_read_all();  // earlier stores have read the staging
-              __syncwarp();
-            }
-            const uint32_t buf = staging + (sub % TMA_OUT) * 4096u;
+          for (int h = 0; h < 2; ++h) {  // 16 rows at a time, in a buffer of their own where there are two
+            const uint32_t to = staging + static_cast<uint32_t>(kBufs > 1 ? h : 0) * 2048u;
+            if (lane == 0) bulk_wait_read<kBufs - 1>();  // the store that used this buffer last has read it
+            __syncwarp();
+            if ((lane >> 4) == h) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const uint32_t chunk = static_cast<uint32_t>(j) ^ (lane & 7u);
-              sts128(buf + lane * 128u + chunk * 16u, packed[sub * 32 + 4 * j], packed[sub * 32 + 4 * j + 1],
-                     packed[sub * 32 + 4 * j + 2], packed[sub * 32 + 4 * j + 3]);
+              for (int j = 0; j < 8; ++j)
+                sts128(to + (lane & 15) * 128u + ((static_cast<uint32_t>(j) ^ (lane & 7u)) * 16u), out[4 * j],
+                       out[4 * j + 1], out[4 * j + 2], out[4 * j + 3]);
             }
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
-              if (col0 + sub * 64 < p.N) tma_store_2d(&map_d, buf, col0 + sub * 64, row0, store_policy);
+              if (row0 + 16 * h < p.rows) tma_store_2d(&map_d, to, col0, row0 + 16 * h, store_policy);
               bulk_commit();
             }
           }
@@ -533,9 +574,8 @@ __global__ void __launch_bounds__(kGroupThreads, 1)
       } else if (mine) {
         uint4* dst = reinterpret_cast<uint4*>(p.D + at);
 #pragma unroll
-        for (int i = 0; i < kHalf / 8; ++i)
-          if (col0 + 8 * i < p.N)
-            dst[i] = make_uint4(packed[4 * i], packed[4 * i + 1], packed[4 * i + 2], packed[4 * i + 3]);
+        for (int j = 0; j < kCols / 8; ++j)
+          if (col0 + 8 * j < p.N) dst[j] = make_uint4(out[4 * j], out[4 * j + 1], out[4 * j + 2], out[4 * j + 3]);
       }
     }
     if constexpr (TMA_OUT > 0) {
@@ -566,11 +606,27 @@ struct GroupedCall {
   const char* who;
 };
 
-template <int CG, int BN, int STAGES, int TMA_OUT, int AM, int MMAS, int NACC>
+// One 16-row x 64-column store box of the 16-bit [rows, N] output, 128-byte swizzled in shared memory.
+int encode_store_map(CUtensorMap* map, void* base, int rows, int N) {
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(N), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(N) * 2};
+  const cuuint32_t box[2] = {64, 16};
+  const cuuint32_t elem[2] = {1, 1};
+  const CUresult r = encode_tiled_fn()(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, base, dims, strides, box, elem,
+                                       CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                       CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled(output) failed with %d", static_cast<int>(r));
+    return B2_ERR_CUDA;
+  }
+  return B2_OK;
+}
+
+template <int CG, int BN, int STAGES, int TMA_OUT, int AM, int MMAS, int NACC, int SETS = 2, int PARTS = 2>
 int launch_grouped(const GroupedCall& c, cudaStream_t stream) {
   using L = GroupedLayout<CG, BN, STAGES, TMA_OUT, AM>;
   constexpr int kBM = AM * CG;
-  auto kernel = nvfp4_grouped_gemm_kernel<CG, BN, STAGES, TMA_OUT, AM, MMAS, NACC>;
+  auto kernel = nvfp4_grouped_gemm_kernel<CG, BN, STAGES, TMA_OUT, AM, MMAS, NACC, SETS, PARTS>;
   GroupedParams p = c.p;
   CUtensorMap map_a, map_b, map_sfa, map_sfb, map_d = {};
   if (int rc = encode_operand_map(&map_a, c.A, p.rows, c.K, AM)) return rc;
@@ -578,16 +634,17 @@ int launch_grouped(const GroupedCall& c, cudaStream_t stream) {
   if (int rc = encode_scale_map(&map_sfa, c.SFA, c.sfa_tiles * 128, c.K, 1)) return rc;
   if (int rc = encode_scale_map(&map_sfb, c.SFB, p.groups * ((p.N + 127) / 128) * 128, c.K, L::kChunks)) return rc;
   if (TMA_OUT > 0) {
-    if (int rc = encode_output_map(&map_d, p.D, p.rows, p.N)) return rc;
+    if (int rc = encode_store_map(&map_d, p.D, p.rows, p.N)) return rc;
   }
   p.k_slabs = (c.K + kBlockK - 1) / kBlockK;
+  p.tiles_m = (p.rows + kBM - 1) / kBM;
   p.tiles_n = (p.N + BN - 1) / BN;
   p.group_n = 8;
   const int sms = device_sm_count();
   if (sms <= 0) return B2_ERR_CUDA;
   // The most row tiles that the groups can have; for one group that is their number.
   const int64_t tiles_m = p.offsets ? p.rows / kBM + static_cast<int64_t>(p.groups < p.rows ? p.groups : p.rows)
-                                    : (p.rows + kBM - 1) / kBM;
+                                    : p.tiles_m;
   const int64_t tiles = tiles_m * p.tiles_n;
   if (tiles > 0x3fffffff) {
     set_error("%s: %lld tiles exceed the tile list's range", c.who, static_cast<long long>(tiles));
@@ -603,12 +660,21 @@ int launch_grouped(const GroupedCall& c, cudaStream_t stream) {
     B2_CUDA_TRY(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !configured[dev].load(std::memory_order_acquire)) {
       B2_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAll));
+      if (PARTS == 4) {
+        // setmaxnreg hands out what the block was launched with: with fewer registers a warpgroup would wait for good.
+        cudaFuncAttributes attributes;
+        B2_CUDA_TRY(cudaFuncGetAttributes(&attributes, kernel));
+        if (attributes.numRegs != kRegsLaunch) {
+          set_error("%s: kernel built with %d registers a thread, %d expected", c.who, attributes.numRegs, kRegsLaunch);
+          return B2_ERR_CUDA;
+        }
+      }
       if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
     }
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(units * CG);
-  cfg.blockDim = dim3(kGroupThreads);
+  cfg.blockDim = dim3(group_threads(SETS, PARTS));
   cfg.dynamicSmemBytes = L::kAll;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -677,8 +743,10 @@ int run_grouped(const GroupedCall& c, cudaStream_t s) {
     case 2: return launch_grouped<1, 64, 7, 0, 128, 2, 1>(c, s);
     case 3: return launch_grouped<1, 128, 6, 0, 128, 2, 1>(c, s);
     case 4: return launch_grouped<1, 128, 6, 0, 128, 1, 2>(c, s);
-    case 5: return launch_grouped<2, 256, 5, 1, 128, 1, 1>(c, s);
-    default: return launch_grouped<2, 128, 6, 1, 128, 1, 2>(c, s);
+    case 5: return launch_grouped<2, 256, 5, 1, 128, 1, 1, 1, 4>(c, s);
+    case 6: return launch_grouped<2, 128, 6, 1, 128, 1, 2>(c, s);
+    case 7: return launch_grouped<1, 128, 8, 0, 32, 1, 2>(c, s);
+    default: return launch_grouped<1, 256, 5, 0, 32, 1, 1, 1, 4>(c, s);
   }
 }
 
@@ -787,7 +855,7 @@ extern "C" int b2_nvfp4_grouped_gemm(const void* A, const void* B, const void* S
 }
 
 extern "C" int b2_nvfp4_grouped_gemm_set_variant(int variant) {
-  if (variant < -1 || variant > 6) {
+  if (variant < -1 || variant > 8) {
     b2::set_error("b2_nvfp4_grouped_gemm_set_variant: unknown variant %d", variant);
     return B2_ERR_INVALID_ARGUMENT;
   }
