@@ -291,9 +291,9 @@ int b2_nvfp4_grouped_gemm(const void* A, const void* B, const void* SFA, const v
                           const int32_t* offsets_dev, const void* bias, void* D, int rows, int groups, int N, int K,
                           int out_dtype, int activation, void* stream);
 
-/* Kernel variant of the following two products' calls (-1: automatic): 0, 1 tiles of 32 rows x 64 columns (two MMA
- * warps / two accumulators in turn), 2 128 x 64, 3 and 4 128 x 128 (two MMA warps / two accumulators), 5 a CTA pair
- * with 256 x 256, 6 a CTA pair with 256 x 128.  Every variant takes every shape. */
+/* Kernel variant of the following calls of the two products (-1: automatic): tiles of 0 32 x 64 (dense, two MMA warps),
+ * 1 32 x 128, 2 128 x 64 (dense, two MMA warps), 3 128 x 128, 4 256 x 256 (a CTA pair), 5 256 x 128 (a CTA pair).  Every
+ * variant takes every shape (grouped calls run 1 for 0 and 3 for 2). */
 int b2_nvfp4_grouped_gemm_set_variant(int variant);
 
 /* Reads and clears the status words of the two products on the current device, as b2_nvfp4_gemm_status. */

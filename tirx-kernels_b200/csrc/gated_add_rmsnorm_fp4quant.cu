@@ -4,10 +4,11 @@
 //   h = c * residual + gate * u                    gate: one row per `rows_per_gate` rows (1 without gate)
 //   y = h16 * rsqrt(mean(h16^2) + eps) * w_pre     the norm before the next block; h16 is h as it is stored
 //
-// h16 is written as the new residual, y in the 16-bit type or quantized to NVFP4 (block scale and values as in
-// add_rmsnorm_fp4quant.cu, one E4M3 scale per 16 values, row-major or in 128 x 4 tiles).  Sums of squares, norms and
+// h16 is written as the new residual, y in the 16-bit type or quantized to NVFP4 (one E4M3 scale per 16 values,
+// gs * max|y| / 6 rounded to nearest, row-major or in 128 x 4 tiles; values y * gs / scale rounded to nearest E2M1).  Sums of squares, norms and
 // h are fp32; h is rounded once, to the type it is stored in, and the second norm uses the rounded value so that it is
-// the norm of what the next block's residual will read.
+// the norm of what the next block's residual will read.  The product of a 16-bit value and a 16-bit weight is exact in
+// fp32, so it is taken first and every value sees one or two roundings in front of its last one.
 //
 // The row stays in registers between the two reductions: x and the residual are read once, h and y written once,
 // which is the floor.  A thread has units of 16 values, one 256-bit access each and, quantized, one scale block.
@@ -31,7 +32,7 @@ struct GatedParams {
   int M, H, units;        // units = H / 16
   int rows_per_gate;
   int sf_pad_cols;        // > 0: 128 x 4 tiles
-  float scale, eps, inv_h;
+  float scale, eps;
 };
 
 __device__ __forceinline__ void ld_256(const void* p, uint32_t (&r)[8]) {
@@ -61,6 +62,11 @@ __device__ __forceinline__ float row_sum(float v, float* red, int warps, int war
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
   return v;
+}
+
+// 1 / sqrt(mean + eps), correctly rounded steps: once per row, and the quantizer's borders see every unit in the last place.
+__device__ __forceinline__ float inverse_root(float sum, const GatedParams& p) {
+  return __frcp_rn(__fsqrt_rn(__fdiv_rn(sum, static_cast<float>(p.H)) + p.eps));
 }
 
 // blockDim = (threads per row, rows per CTA); more than one row per CTA only with 32 threads per row.  V units per thread.
@@ -96,7 +102,7 @@ __global__ void __launch_bounds__(1024) gated_add_rmsnorm_kernel(const __grid_co
         }
       }
     }
-    rstd = rsqrtf(fmaf(row_sum(sum, red[0], warps, warp, lane), p.inv_h, p.eps));
+    rstd = inverse_root(row_sum(sum, red[0], warps, warp, lane), p);
   }
   const uint8_t* gate = p.gate ? p.gate + static_cast<int64_t>(row / p.rows_per_gate) * p.H * 2 : nullptr;
   float sum = 0.0f;
@@ -112,7 +118,7 @@ __global__ void __launch_bounds__(1024) gated_add_rmsnorm_kernel(const __grid_co
         float2 v = unpack2<Tag>(x[j][i]);
         if (p.w_post) {
           const float2 f = unpack2<Tag>(w[i]);
-          v = make_float2(v.x * rstd * f.x, v.y * rstd * f.y);
+          v = make_float2(v.x * f.x * rstd, v.y * f.y * rstd);
         }
         if (gate) {
           const float2 f = unpack2<Tag>(g[i]);
@@ -127,9 +133,8 @@ __global__ void __launch_bounds__(1024) gated_add_rmsnorm_kernel(const __grid_co
       st_256(p.residual_out + at + static_cast<int64_t>(u) * 32, h[j]);
     }
   }
-  rstd = rsqrtf(fmaf(row_sum(sum, red[1], warps, warp, lane), p.inv_h, p.eps));
+  rstd = inverse_root(row_sum(sum, red[1], warps, warp, lane), p);
   const float gs = QUANT ? __ldg(p.gs) : 0.0f;
-  const float rcp6 = rcp_approx_ftz(6.0f);
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     const int u = t + j * blockDim.x;
@@ -140,21 +145,21 @@ __global__ void __launch_bounds__(1024) gated_add_rmsnorm_kernel(const __grid_co
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float2 f = unpack2<Tag>(h[j][i]), g = unpack2<Tag>(w[i]);
-        v[2 * i] = f.x * rstd * g.x;
-        v[2 * i + 1] = f.y * rstd * g.y;
+        v[2 * i] = f.x * g.x;
+        v[2 * i + 1] = f.y * g.y;
       }
       if constexpr (!QUANT) {
         uint32_t o[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = pack_from_f32<Tag>(v[2 * i], v[2 * i + 1]);
+        for (int i = 0; i < 8; ++i) o[i] = pack_from_f32<Tag>(v[2 * i] * rstd, v[2 * i + 1] * rstd);
         st_256(p.y + at + static_cast<int64_t>(u) * 32, o);
       } else {
         float amax = 0.0f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) amax = max_f32(amax, fabsf(v[i]));
-        const uint32_t code = cvt_f32_to_e4m3(min_f32(mul_f32(mul_f32(gs, amax), rcp6), 448.0f)) & 0xFFu;
+        const uint32_t code = cvt_f32_to_e4m3(min_f32(__fdiv_rn(gs * (amax * rstd), 6.0f), 448.0f)) & 0xFFu;
         const float d = e4m3_to_f32(code);
-        const float out_scale = d == 0.0f ? 0.0f : mul_f32(rcp_approx_ftz(d), gs);
+        const float out_scale = d == 0.0f ? 0.0f : __fdiv_rn(gs, d) * rstd;
         float lo[8], hi[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -248,7 +253,6 @@ extern "C" int b2_gated_add_rmsnorm_fp4quant(const void* x, const void* residual
   p.sf_pad_cols = quantize && swizzled ? (p.units + 3) / 4 * 4 : 0;
   p.scale = residual_scale;
   p.eps = eps;
-  p.inv_h = 1.0f / static_cast<float>(H);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (in_dtype == B2_DTYPE_F16) return dispatch_gated<F16Tag>(p, quantize != 0, s);
   return dispatch_gated<BF16Tag>(p, quantize != 0, s);

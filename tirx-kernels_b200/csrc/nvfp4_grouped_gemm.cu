@@ -68,9 +68,10 @@ struct Tile {
 
 // Work item t -> its tile.  starts[g] is the number of row tiles in front of group g; among groups without rows,
 // which share a start, bisection ends at the last one, the one that has the tile.
+template <bool GROUPED>
 __device__ __forceinline__ Tile find_tile(const GroupedParams& p, const int* starts, const int* rows, int t) {
   Tile r;
-  if (!p.offsets) {
+  if constexpr (!GROUPED) {
     r.group = 0;
     r.first = 0;
     r.last = p.rows;
@@ -119,50 +120,72 @@ __device__ __forceinline__ uint4 load_residual(const uint16_t* p) {
   asm volatile("ld.global.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
   return r;
 }
+// A load whose value nobody uses: what it leaves behind is the line in L1.
+__device__ __forceinline__ void touch(const uint16_t* p) {
+  asm volatile("{ .reg .b32 a, b, c, d; ld.global.nc.v4.b32 {a, b, c, d}, [%0]; }" ::"l"(p));
+}
 __device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
-// 8 accumulator columns of one row -> 4 packed words of the output.  `bias` is null or points at the first of the
-// columns, `add` says whether `r` is a part of the residual.  Eight at a time: the raw accumulator takes up to 64
-// registers, little else may live beside it.
-template <typename Tag>
-__device__ __forceinline__ void finish8(int act, float alpha, const uint16_t* bias, bool add, uint4 r, const uint32_t* v,
-                                        uint32_t* out) {
-  float f[8];
+// ---- the epilogue's steps, each over all of a warp's columns of one row, in place --------------------------------------
+// One step after another, with the choice of activation or type outside the loop: what a call does not use it does not
+// fetch.  With the choices inside, eight columns at a time, the instructions that a short launch jumped over cost it
+// 1 to 2 us (16 x 8192 x 8192 11.4 us for 10.6).
+template <typename Tag, int COLS>
+__device__ __forceinline__ void add_bias(const uint16_t* bias, int left, uint32_t* v) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(v[i]) * alpha;
-  if (bias) {
-    const uint4 b = __ldg(reinterpret_cast<const uint4*>(bias));
-    const uint32_t w[4] = {b.x, b.y, b.z, b.w};
+  for (int c = 0; c < COLS / 8; ++c) {
+    if (8 * c < left) {
+      const uint4 b = __ldg(reinterpret_cast<const uint4*>(bias + 8 * c));
+      const uint32_t w[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f[2 * i] += unpack_lo<Tag>(w[i]);
-      f[2 * i + 1] += unpack_hi<Tag>(w[i]);
+      for (int i = 0; i < 4; ++i) {
+        v[8 * c + 2 * i] = __float_as_uint(__uint_as_float(v[8 * c + 2 * i]) + unpack_lo<Tag>(w[i]));
+        v[8 * c + 2 * i + 1] = __float_as_uint(__uint_as_float(v[8 * c + 2 * i + 1]) + unpack_hi<Tag>(w[i]));
+      }
     }
   }
+}
+template <int COLS>
+__device__ __forceinline__ void activate(int act, uint32_t* v) {
   if (act == B2_ACT_SILU || act == B2_ACT_GELU_TANH) {
     const float c1 = act == B2_ACT_SILU ? 1.4426950408889634f : 2.3022081983375f;
     const float c2 = act == B2_ACT_SILU ? 0.0f : 0.10294324f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = gate_sigmoid(f[i], c1, c2);
+    for (int i = 0; i < COLS; ++i) v[i] = __float_as_uint(gate_sigmoid(__uint_as_float(v[i]), c1, c2));
   } else if (act == B2_ACT_GELU) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = gelu_erf(f[i]);
-  } else if (act == B2_ACT_RELU) {
+    for (int i = 0; i < COLS; ++i) v[i] = __float_as_uint(gelu_erf(__uint_as_float(v[i])));
+  } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = f[i] < 0.0f ? 0.0f : f[i];  // a NaN stays one
+    for (int i = 0; i < COLS; ++i) v[i] = __uint_as_float(v[i]) < 0.0f ? 0u : v[i];  // ReLU; a NaN stays one
   }
-  if (add) {
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+}
+template <typename Tag>
+__device__ __forceinline__ void add8(uint4 r, uint32_t* v) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f[2 * i] += unpack_lo<Tag>(w[i]);
-      f[2 * i + 1] += unpack_hi<Tag>(w[i]);
-    }
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __float_as_uint(__uint_as_float(v[2 * i]) + unpack_lo<Tag>(w[i]));
+    v[2 * i + 1] = __float_as_uint(__uint_as_float(v[2 * i + 1]) + unpack_hi<Tag>(w[i]));
   }
+}
+// The one rounding: words 0 .. N/2 - 1 become the packed columns.
+template <typename Tag, int N>
+__device__ __forceinline__ void pack(uint32_t* v) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) out[i] = pack_from_f32<Tag>(f[2 * i], f[2 * i + 1]);
+  for (int i = 0; i < N / 2; ++i) v[i] = pack_from_f32<Tag>(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
 }
 
+__device__ __forceinline__ uint4 lds128_vec(uint32_t addr) {
+  uint32_t r[4];
+  lds128(addr, r);
+  return make_uint4(r[0], r[1], r[2], r[3]);
+}
+// Asks L2 for a box of a tensor map.
+__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, int y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y)
+               : "memory");
+}
 __device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
@@ -193,11 +216,12 @@ constexpr int group_threads(int sets, int parts) { return 32 * (4 + 4 * sets + 4
 constexpr int kRegsLaunch = 80, kRegsIssue = 56, kRegsScale = 40, kRegsEpilogue = 96;
 static_assert(kRegsIssue + kRegsScale + 4 * kRegsEpilogue <= 6 * kRegsLaunch, "no warpgroup waits for registers that nobody gives");
 
-template <int CG, int BN, int STAGES, int TMA_OUT, int AM, int MMAS, int NACC, int SETS, int PARTS>
+template <bool GROUPED, int CG, int BN, int STAGES, int TMA_OUT, int AM, int MMAS, int NACC, int SETS, int PARTS>
 __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
     nvfp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                               const __grid_constant__ CUtensorMap map_sfa, const __grid_constant__ CUtensorMap map_sfb,
-                              const __grid_constant__ CUtensorMap map_d, const __grid_constant__ GroupedParams p) {
+                              const __grid_constant__ CUtensorMap map_d, const __grid_constant__ CUtensorMap map_r,
+                              const __grid_constant__ GroupedParams p) {
   using L = GroupedLayout<CG, BN, STAGES, TMA_OUT, AM>;
   static_assert(MMAS == 1 || (CG == 1 && TMA_OUT == 0), "the second MMA warp exists for single-CTA tiles");
   static_assert(CG == 1 || AM == kBlockM, "pairs load all rows");
@@ -225,7 +249,8 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
   auto empty_bar = [&](int s) { return bar_base + 8u * (2 * STAGES + s); };
   auto acc_full_bar = [&](int a) { return bar_base + 8u * (3 * STAGES + a); };
   auto acc_empty_bar = [&](int a) { return bar_base + 8u * (3 * STAGES + NACC + a); };
-  static_assert((3 * STAGES + 2 * NACC) * 8 + 16 <= L::kBarrierBytes, "barrier area");
+  constexpr int kResBarOffset = (3 * STAGES + 2 * NACC) * 8 + 16;  // residual landed, per epilogue warp
+  static_assert(kResBarOffset + 32 * PARTS <= L::kBarrierBytes, "barrier area");
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_gen + L::kRingBytes + 8 * (3 * STAGES + 2 * NACC));
   volatile uint32_t* abort_flag = tmem_slot + 1;
   int* starts = reinterpret_cast<int*>(smem_gen + L::kTable);  // [groups + 1] row tiles in front of a group
@@ -250,6 +275,8 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
       mbar_init(acc_full_bar(a), MMAS);
       mbar_init(acc_empty_bar(a), 4 * PARTS * CG);  // one arrive per epilogue warp of every CTA in the group
     }
+    if constexpr (TMA_OUT > 0)
+      for (int w = 0; w < 4 * PARTS; ++w) mbar_init(bar_base + kResBarOffset + 8u * w, 1);
     *abort_flag = 0u;
     fence_barrier_init();
     prefetch_tmap(&map_a);
@@ -261,46 +288,49 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
     tmem_alloc<CG>(smem_u32(tmem_slot), kTmemCols);
     tmem_relinquish<CG>();
   }
-  // Dependent launch as in nvfp4_gemm.cu: nothing in front of this wait touches global memory.
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (p.offsets && warp == kGWarpMma2) {
-    int tiles = 0;  // row tiles in front of the 32 groups of this step
-    for (int g0 = 0; g0 < p.groups; g0 += 32) {
-      const int g = g0 + lane;
-      int first = 0, last = 0;
-      if (g < p.groups) {
-        // Offsets that are not ascending or leave [0, rows] are brought back into it: no access leaves A or D.
-        first = min(max(__ldg(p.offsets + g), 0), p.rows);
-        last = min(max(__ldg(p.offsets + g + 1), first), p.rows);
-      }
-      const int mine = (last - first + kBM - 1) / kBM;
-      int sum = mine;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, sum, d);
-        if (lane >= d) sum += up;
-      }
-      if (g < p.groups) {
-        starts[g] = tiles + sum - mine;
-        group_rows[g] = first;
-        if (g == p.groups - 1) {
-          starts[g + 1] = tiles + sum;
-          group_rows[g + 1] = last;
-        }
-      }
-      tiles += __shfl_sync(0xffffffffu, sum, 31);
-    }
-  }
   tc_fence_before();
   __syncthreads();
   if constexpr (CG == 2) cluster_sync_all();
   tc_fence_after();
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t tmem_base = kWarpWide ? __shfl_sync(0xffffffffu, *tmem_slot, 0) : *tmem_slot;
+  // Dependent launch as in nvfp4_gemm.cu: nothing in front of this wait touches global memory.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if constexpr (GROUPED) {
+    if (warp == kGWarpMma2) {
+      int tiles = 0;  // row tiles in front of the 32 groups of this step
+      for (int g0 = 0; g0 < p.groups; g0 += 32) {
+        const int g = g0 + lane;
+        int first = 0, last = 0;
+        if (g < p.groups) {
+          // Offsets that are not ascending or leave [0, rows] are brought back into it: no access leaves A or D.
+          first = min(max(__ldg(p.offsets + g), 0), p.rows);
+          last = min(max(__ldg(p.offsets + g + 1), first), p.rows);
+        }
+        const int mine = (last - first + kBM - 1) / kBM;
+        int sum = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+          const int up = __shfl_up_sync(0xffffffffu, sum, d);
+          if (lane >= d) sum += up;
+        }
+        if (g < p.groups) {
+          starts[g] = tiles + sum - mine;
+          group_rows[g] = first;
+          if (g == p.groups - 1) {
+            starts[g + 1] = tiles + sum;
+            group_rows[g + 1] = last;
+          }
+        }
+        tiles += __shfl_sync(0xffffffffu, sum, 31);
+      }
+    }
+    __syncthreads();
+  }
   // What the issuing warps compute from shared memory is made uniform by a shuffle, or the compiler would keep their
   // loops' state out of uniform registers (nvfp4_gemm.cu).
   auto uniform = [](int v) { return kWarpWide ? __shfl_sync(0xffffffffu, v, 0) : v; };
-  const int num_tiles = p.offsets ? uniform(starts[p.groups]) * p.tiles_n : p.tiles_m * p.tiles_n;
+  const int num_tiles = GROUPED ? uniform(starts[p.groups]) * p.tiles_n : p.tiles_m * p.tiles_n;
   const int k_slabs = p.k_slabs;
 
   // The waits of the issuing roles: of the whole warp with one outcome, or of lane 0.
@@ -308,6 +338,11 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
     const bool ok = wait_or_abort(bar, phase, ctx, code);
     if constexpr (kWarpWide) return __all_sync(0xffffffffu, ok) != 0;
     else return ok;
+  };
+  // The epilogue's waits: one outcome for all lanes, since the warp goes on with __syncwarp.  (The scale warps poll
+  // converged as in nvfp4_gemm.cu: the vote would cost them 4 % of a decode product, once per slab.)
+  auto warp_wait = [&](uint32_t bar, uint32_t phase, uint32_t code) {
+    return __all_sync(0xffffffffu, wait_or_abort(bar, phase, ctx, code)) != 0;
   };
   auto issues = [&] { return kWarpWide ? elect_one() : true; };
 
@@ -322,7 +357,7 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
       uint32_t phase = 0;
       bool alive = true;
       for (int t = unit; t < num_tiles && alive; t += num_units) {
-        const Tile tile = find_tile(p, starts, group_rows, t);
+        const Tile tile = find_tile<GROUPED>(p, starts, group_rows, t);
         const int row_a = uniform(tile.first + tile.tm * kBM) + static_cast<int>(rank) * kBlockM;
         const int row_b = uniform(tile.group * p.N + tile.tn * BN) + static_cast<int>(rank) * L::kBRows;
         for (int ks = 0; ks < k_slabs; ++ks) {
@@ -348,7 +383,7 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
       uint32_t phase = 0;
       bool alive = true;
       for (int t = unit; t < num_tiles && alive; t += num_units) {
-        const Tile tile = find_tile(p, starts, group_rows, t);
+        const Tile tile = find_tile<GROUPED>(p, starts, group_rows, t);
         const int sfa_tile = uniform((tile.first >> 7) + tile.group + ((tile.tm * kBM) >> 7)) + static_cast<int>(rank);
         const int sfb_tile = uniform(tile.group * sfb_tiles + (tile.tn * BN) / 128);
         for (int ks = 0; ks < k_slabs; ++ks) {
@@ -378,7 +413,7 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
         tc_fence_after();
         // A 64-wide tile uses half of a 128-row scale chunk of B: the upper half starts two columns in.
         uint32_t sfb_half = 0;
-        if constexpr (BN == 64) sfb_half = static_cast<uint32_t>(find_tile(p, starts, group_rows, t).tn & 1) * 2u;
+        if constexpr (BN == 64) sfb_half = static_cast<uint32_t>(find_tile<GROUPED>(p, starts, group_rows, t).tn & 1) * 2u;
         const uint32_t acc_tmem = tmem_base + static_cast<uint32_t>((acc * MMAS + me) * BN);
         int stage = (slab0 + me) % STAGES;
         uint32_t phase = static_cast<uint32_t>((slab0 + me) / STAGES) & 1u;
@@ -435,7 +470,7 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
     for (int n = 0; n < total_slabs; ++n) {
       if constexpr (AM == 32) {
         if (tile_slabs == 0) {
-          part = find_tile(p, starts, group_rows, t).tm & 3;
+          part = find_tile<GROUPED>(p, starts, group_rows, t).tm & 3;
           t += num_units;
           tile_slabs = k_slabs;
         }
@@ -448,10 +483,21 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
       const uint32_t sfa_smem = smem_base + stage * L::kStageBytes + L::kABytes + L::kBBytes + lane * 16;
       const uint32_t sfb_smem = sfa_smem + L::kSfaBytes;
       const uint32_t dst = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + kAccCols + stage * L::kSfCols;
-      // Sixteen words at a time: with a slab's 48 in flight the warp would need registers that the epilogue wants.
-      uint32_t a[16];
+      // The whole slab's words at once, or, where the epilogue wants the registers, sixteen at a time.
+      auto load_b = [&](int c, uint32_t* b) {  // words 16 c .. 16 c + 15 of [kb][chunk][4]
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int word = 4 * c + i;
+          lds128(sfb_smem + ((word % L::kChunks) * 4 + word / L::kChunks) * 512, b + 4 * i);
+        }
+      };
+      uint32_t a[16], ahead[kMoveRegisters ? 1 : 16 * L::kChunks];
 #pragma unroll
       for (int kb = 0; kb < 4; ++kb) lds128(sfa_smem + kb * 512, a + 4 * kb);
+      if constexpr (!kMoveRegisters) {
+#pragma unroll
+        for (int c = 0; c < L::kChunks; ++c) load_b(c, ahead + 16 * c);
+      }
       if constexpr (AM == 32) {
 #pragma unroll
         for (int kb = 0; kb < 4; ++kb) {
@@ -461,14 +507,14 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
       }
       tmem_st_32x32_x16(dst, a);
 #pragma unroll
-      for (int c = 0; c < L::kChunks; ++c) {  // words 16 c .. 16 c + 15 of [kb][chunk][4]
-        uint32_t b[16];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int word = 4 * c + i;
-          lds128(sfb_smem + ((word % L::kChunks) * 4 + word / L::kChunks) * 512, b + 4 * i);
+      for (int c = 0; c < L::kChunks; ++c) {
+        if constexpr (kMoveRegisters) {
+          uint32_t b[16];
+          load_b(c, b);
+          tmem_st_32x32_x16(dst + 16 + 16 * c, b);
+        } else {
+          tmem_st_32x32_x16(dst + 16 + 16 * c, ahead + 16 * c);
         }
-        tmem_st_32x32_x16(dst + 16 + 16 * c, b);
       }
       tmem_st_wait();
       tc_fence_before();
@@ -491,10 +537,12 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
     constexpr int kBufs = TMA_OUT > 0 ? L::kStagingBytes / (4 * PARTS * 2048) : 1;
     static_assert(kBufs == 1 || kBufs == 2, "store buffers");
     const uint32_t staging = smem_base + STAGES * L::kStageBytes + static_cast<uint32_t>(warp - kWarpEpi0) * kBufs * 2048u;
+    const uint32_t res_bar = bar_base + kResBarOffset + 8u * static_cast<uint32_t>(warp - kWarpEpi0);
+    uint32_t res_phase = 0;
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int t = unit; t < num_tiles; t += num_units) {
-      const Tile tile = find_tile(p, starts, group_rows, t);
+      const Tile tile = find_tile<GROUPED>(p, starts, group_rows, t);
       const float alpha = __ldg(p.alpha + tile.group);
       const int in_tile = static_cast<int>(rank) * kBlockM + quarter * 32;  // first row of this warp in the tile
       const int row0 = tile.first + tile.tm * kBM + in_tile;
@@ -505,8 +553,29 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
       const int64_t at = static_cast<int64_t>(row) * p.N + col0;
       const uint16_t* bias = p.bias ? p.bias + static_cast<int64_t>(tile.group) * p.N + col0 : nullptr;
       const uint16_t* residual = p.residual && mine ? p.residual + at : nullptr;
-      if (residual) prefetch_l2(residual);
-      if (!wait_or_abort(acc_full_bar(acc), acc_phase, ctx, 4u)) break;
+      if constexpr (TMA_OUT > 0) {
+        // The residual comes by the TMA into the staging buffers, half of the rows at a time (both halves at once
+        // where there are two buffers); row-strided loads of it took 8192 x 8192 x 8192 from 199 to 277 us.
+        if (any && p.residual && lane == 0) {
+          bulk_wait_read<0>();  // the stores of the last tile have read the buffers
+          mbar_expect_tx(res_bar, 2048u * kBufs);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (h < kBufs) tma_load_2d<1>(staging + h * 2048u, &map_r, col0, row0 + 16 * h, res_bar);
+            else tma_prefetch_2d(&map_r, col0, row0 + 16 * h);
+          }
+        }
+      } else if (residual && kCols == 64) {
+        prefetch_l2(residual);
+      }
+      uint4 early[4];  // 32 columns leave room for the residual while the products run
+      if constexpr (kCols == 32) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (residual && col0 + 8 * c < p.N) early[c] = load_residual(residual + 8 * c);
+      }
+      if (bias && any && lane < kCols / 8 && col0 + 8 * lane < p.N) touch(bias + 8 * lane);  // into L1
+      if (!warp_wait(acc_full_bar(acc), acc_phase, 4u)) break;
       tc_fence_after();
       uint32_t v[kCols];
       if (any) {
@@ -515,7 +584,7 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
 #pragma unroll
         for (int c0 = 0; c0 < kCols; c0 += 32)
           tmem_ld_32x32(acc_tmem + c0, *reinterpret_cast<uint32_t(*)[32]>(v + c0));
-        tmem_ld_wait();
+        if (MMAS == 1 || !two) tmem_ld_wait();
         if constexpr (MMAS == 2) {
           if (two) {
 #pragma unroll
@@ -539,17 +608,67 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
       if (!any) continue;
       // The TMA clips rows behind the last row and columns behind N, but knows nothing of groups.
       const bool by_tma = TMA_OUT > 0 && (row0 + 32 <= tile.last || tile.last == p.rows);
-      uint32_t* const out = v;  // packed words take the place of accumulators that are done
-      uint4 next = make_uint4(0u, 0u, 0u, 0u);  // the residual's part of the next eight columns, on its way
-      if (residual) next = load_residual(residual);
+      const int left = p.N - col0;
 #pragma unroll
-      for (int c0 = 0; c0 < kCols; c0 += 8) {
-        const uint4 r = next;
-        if (residual && c0 + 8 < kCols && col0 + c0 + 8 < p.N) next = load_residual(residual + c0 + 8);
-        const uint16_t* b = bias && col0 + c0 < p.N ? bias + c0 : nullptr;
-        if (p.fp16) finish8<F16Tag>(p.act, alpha, b, residual != nullptr, r, v + c0, out + c0 / 2);
-        else finish8<BF16Tag>(p.act, alpha, b, residual != nullptr, r, v + c0, out + c0 / 2);
+      for (int i = 0; i < kCols; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
+      if (bias) {
+        if (p.fp16) add_bias<F16Tag, kCols>(bias, left, v);
+        else add_bias<BF16Tag, kCols>(bias, left, v);
       }
+      if (p.act != B2_ACT_NONE) activate<kCols>(p.act, v);
+      if (TMA_OUT > 0 && p.residual) {
+        if constexpr (TMA_OUT > 0) {
+          bool landed = true;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t here = staging + static_cast<uint32_t>(kBufs > 1 ? h : 0) * 2048u + (lane & 15) * 128u;
+            if (h >= kBufs && lane == 0) {
+              bulk_wait_read<0>();  // the first half's store has read the buffer
+              mbar_expect_tx(res_bar, 2048u);
+              tma_load_2d<1>(staging, &map_r, col0, row0 + 16, res_bar);
+            }
+            landed = warp_wait(res_bar, res_phase, 6u);
+            if (!landed) break;
+            if (kBufs == 1 || h == 1) res_phase ^= 1u;
+            if ((lane >> 4) == h) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const uint32_t at_j = here + ((static_cast<uint32_t>(j) ^ (lane & 7u)) * 16u);
+                uint32_t* o = v + 8 * j;
+                if (p.fp16) {
+                  add8<F16Tag>(lds128_vec(at_j), o);
+                  pack<F16Tag, 8>(o);
+                } else {
+                  add8<BF16Tag>(lds128_vec(at_j), o);
+                  pack<BF16Tag, 8>(o);
+                }
+                sts128(at_j, o[0], o[1], o[2], o[3]);
+              }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              if (row0 + 16 * h < p.rows)
+                tma_store_2d(&map_d, staging + static_cast<uint32_t>(kBufs > 1 ? h : 0) * 2048u, col0, row0 + 16 * h, store_policy);
+              bulk_commit();
+            }
+          }
+          if (!landed) break;
+        }
+        continue;
+      }
+      if (residual) {
+#pragma unroll
+        for (int c = 0; c < kCols / 8; ++c) {
+          if (8 * c < left) {
+            const uint4 r = kCols == 32 ? early[c % 4] : load_residual(residual + 8 * c);
+            if (p.fp16) add8<F16Tag>(r, v + 8 * c);
+            else add8<BF16Tag>(r, v + 8 * c);
+          }
+        }
+      }
+      if (p.fp16) pack<F16Tag, kCols>(v);
+      else pack<BF16Tag, kCols>(v);
       if (TMA_OUT > 0 && by_tma) {
         if constexpr (TMA_OUT > 0) {
 #pragma unroll
@@ -560,8 +679,8 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
             if ((lane >> 4) == h) {
 #pragma unroll
               for (int j = 0; j < 8; ++j)
-                sts128(to + (lane & 15) * 128u + ((static_cast<uint32_t>(j) ^ (lane & 7u)) * 16u), out[4 * j],
-                       out[4 * j + 1], out[4 * j + 2], out[4 * j + 3]);
+                sts128(to + (lane & 15) * 128u + ((static_cast<uint32_t>(j) ^ (lane & 7u)) * 16u), v[4 * j], v[4 * j + 1],
+                       v[4 * j + 2], v[4 * j + 3]);
             }
             fence_proxy_async_smem();
             __syncwarp();
@@ -575,7 +694,7 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
         uint4* dst = reinterpret_cast<uint4*>(p.D + at);
 #pragma unroll
         for (int j = 0; j < kCols / 8; ++j)
-          if (col0 + 8 * j < p.N) dst[j] = make_uint4(out[4 * j], out[4 * j + 1], out[4 * j + 2], out[4 * j + 3]);
+          if (col0 + 8 * j < p.N) dst[j] = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
       }
     }
     if constexpr (TMA_OUT > 0) {
@@ -622,19 +741,21 @@ int encode_store_map(CUtensorMap* map, void* base, int rows, int N) {
   return B2_OK;
 }
 
-template <int CG, int BN, int STAGES, int TMA_OUT, int AM, int MMAS, int NACC, int SETS = 2, int PARTS = 2>
+template <bool GROUPED, int CG, int BN, int STAGES, int TMA_OUT, int AM, int MMAS, int NACC, int SETS = 2, int PARTS = 2>
 int launch_grouped(const GroupedCall& c, cudaStream_t stream) {
   using L = GroupedLayout<CG, BN, STAGES, TMA_OUT, AM>;
   constexpr int kBM = AM * CG;
-  auto kernel = nvfp4_grouped_gemm_kernel<CG, BN, STAGES, TMA_OUT, AM, MMAS, NACC, SETS, PARTS>;
+  auto kernel = nvfp4_grouped_gemm_kernel<GROUPED, CG, BN, STAGES, TMA_OUT, AM, MMAS, NACC, SETS, PARTS>;
   GroupedParams p = c.p;
-  CUtensorMap map_a, map_b, map_sfa, map_sfb, map_d = {};
+  CUtensorMap map_a, map_b, map_sfa, map_sfb, map_d = {}, map_r = {};
   if (int rc = encode_operand_map(&map_a, c.A, p.rows, c.K, AM)) return rc;
   if (int rc = encode_operand_map(&map_b, c.B, p.groups * p.N, c.K, L::kBRows)) return rc;
   if (int rc = encode_scale_map(&map_sfa, c.SFA, c.sfa_tiles * 128, c.K, 1)) return rc;
   if (int rc = encode_scale_map(&map_sfb, c.SFB, p.groups * ((p.N + 127) / 128) * 128, c.K, L::kChunks)) return rc;
   if (TMA_OUT > 0) {
     if (int rc = encode_store_map(&map_d, p.D, p.rows, p.N)) return rc;
+    if (p.residual)
+      if (int rc = encode_store_map(&map_r, const_cast<uint16_t*>(p.residual), p.rows, p.N)) return rc;
   }
   p.k_slabs = (c.K + kBlockK - 1) / kBlockK;
   p.tiles_m = (p.rows + kBM - 1) / kBM;
@@ -643,8 +764,8 @@ int launch_grouped(const GroupedCall& c, cudaStream_t stream) {
   const int sms = device_sm_count();
   if (sms <= 0) return B2_ERR_CUDA;
   // The most row tiles that the groups can have; for one group that is their number.
-  const int64_t tiles_m = p.offsets ? p.rows / kBM + static_cast<int64_t>(p.groups < p.rows ? p.groups : p.rows)
-                                    : p.tiles_m;
+  const int64_t tiles_m = GROUPED ? p.rows / kBM + static_cast<int64_t>(p.groups < p.rows ? p.groups : p.rows)
+                                  : p.tiles_m;
   const int64_t tiles = tiles_m * p.tiles_n;
   if (tiles > 0x3fffffff) {
     set_error("%s: %lld tiles exceed the tile list's range", c.who, static_cast<long long>(tiles));
@@ -689,7 +810,7 @@ int launch_grouped(const GroupedCall& c, cudaStream_t stream) {
   attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
   ++cfg.numAttrs;
-  B2_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, map_a, map_b, map_sfa, map_sfb, map_d, p));
+  B2_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, map_a, map_b, map_sfa, map_sfb, map_d, map_r, p));
   return B2_OK;
 }
 
@@ -717,37 +838,56 @@ int grouped_status_words(uint32_t** out) {
 
 std::atomic<int> g_grouped_variant{-1};  // test hook: -1 = automatic
 
-// The kernel for `rows` rows in `groups` groups (numbering of b2_nvfp4_grouped_gemm_set_variant).
-int choose_grouped_variant(int rows, int groups, int N, int sms) {
-  const int64_t mean = (static_cast<int64_t>(rows) + groups - 1) / groups;
-  if (mean <= 32) return groups == 1 && (N + 63) / 64 <= sms ? 0 : 1;
-  if (groups == 1 && rows <= 128 && (N + 63) / 64 <= sms) return 2;
-  const int64_t tiles = ((mean + 127) / 128) * groups * ((N + 127) / 128);
-  if (groups == 1 && tiles <= sms) return 3;
-  if (mean <= 128) return 4;
-  if (groups == 1) {
-    const int64_t pairs = (mean + 255) / 256 * ((N + 255) / 256);
-    return pairs * 2 <= sms / 2 ? 6 : 5;
+// The kernel for `rows` rows in `groups` groups (numbering of b2_nvfp4_grouped_gemm_set_variant).  Times on B200, back
+// to back launches from a CUDA graph, us:
+//   dense     32 x 64, 2 MMA warps   all of N in one wave of 64-wide tiles: 16 x 8192 x 8192 9.9 (32 x 128: 12.6)
+//             32 x 128               more: 16 x 28672 x 8192 26.8 (32 x 64: 31.9)
+//             128 x 64, 2 MMA warps  one wave of them: 1024^3 4.8 (256 x 128: 5.8), 200 x 4096 x 4096 7.1 (8.0)
+//             128 x 128              more columns, at most 128 rows: 64 x 28672 x 8192 29.1 (256 x 256: 31.4)
+//             256 x 128              one wave of them: 256 x 8192 x 8192 11.2 (256 x 256: 15.0, 128 x 128: 14.4)
+//             256 x 256              the rest: 2048 x 4096 x 4096 18.1 (256 x 128: 19.9)
+//   grouped   32 x 128               mean of 16 rows: 1024 rows of 64, N=2048, K=4096 60.2 (128 x 128: 61.4); 8 rows 11.9 (15.1)
+//             128 x 128              mean of 64 rows: 4096 of 64, N=K=2048 39.3 (256 x 256: 41.8), or about one wave of
+//                                    them: 777 of 7, N=1352, K=1088 8.2 (9.4)
+//             256 x 128              at most two waves of 256 x 256: 1024 of 8, N=K=2048 10.6 (256 x 256: 13.5, 128 x 128: 13.1)
+//             256 x 256              the rest: 16384 of 32, N=2816, K=2048 68.4 (256 x 128: 78.9)
+int choose_grouped_variant(int rows, int groups, bool grouped, int N, int sms) {
+  const int64_t n64 = (N + 63) / 64, n128 = (N + 127) / 128, n256 = (N + 255) / 256;
+  if (!grouped) {
+    const int64_t m128 = (rows + 127) / 128, m256 = (rows + 255) / 256;
+    if (rows <= 32) return n64 <= sms ? 0 : 1;
+    if (m128 * n64 <= sms) return 2;
+    if (rows <= 128) return 3;
+    return m256 * n128 <= sms / 2 ? 5 : 4;
   }
-  return 5;
+  // The groups' sizes are known on the device alone: a group's last tile is taken to be half full.
+  const int64_t mean = (static_cast<int64_t>(rows) + groups - 1) / groups;
+  if (mean <= 16) return 1;
+  if (mean <= 64 || (2 * (rows / 128) + groups) * n128 <= 2 * sms) return 3;
+  return (2 * (rows / 256) + groups) * n256 <= 2 * sms ? 5 : 4;
+}
+
+// The two-MMA-warp kernels are for one tile per CTA, which only a dense product knows to have.
+template <bool GROUPED>
+int run_variant(int variant, const GroupedCall& c, cudaStream_t s) {
+  switch (variant) {
+    case 0:
+      if constexpr (!GROUPED) return launch_grouped<false, 1, 64, 11, 0, 32, 2, 1>(c, s);
+    case 1: return launch_grouped<GROUPED, 1, 128, 8, 0, 32, 1, 2>(c, s);
+    case 2:
+      if constexpr (!GROUPED) return launch_grouped<false, 1, 64, 7, 0, 128, 2, 1>(c, s);
+    case 3: return launch_grouped<GROUPED, 1, 128, 6, 0, 128, 1, 2>(c, s);
+    case 4: return launch_grouped<GROUPED, 2, 256, 5, 1, 128, 1, 1, 1, 4>(c, s);
+    default: return launch_grouped<GROUPED, 2, 128, 6, 1, 128, 1, 2>(c, s);
+  }
 }
 
 int run_grouped(const GroupedCall& c, cudaStream_t s) {
   const int sms = device_sm_count();
   if (sms <= 0) return B2_ERR_CUDA;
   int variant = g_grouped_variant.load(std::memory_order_relaxed);
-  if (variant < 0) variant = choose_grouped_variant(c.p.rows, c.p.groups, c.p.N, sms);
-  switch (variant) {
-    case 0: return launch_grouped<1, 64, 11, 0, 32, 2, 1>(c, s);
-    case 1: return launch_grouped<1, 64, 11, 0, 32, 1, 2>(c, s);
-    case 2: return launch_grouped<1, 64, 7, 0, 128, 2, 1>(c, s);
-    case 3: return launch_grouped<1, 128, 6, 0, 128, 2, 1>(c, s);
-    case 4: return launch_grouped<1, 128, 6, 0, 128, 1, 2>(c, s);
-    case 5: return launch_grouped<2, 256, 5, 1, 128, 1, 1, 1, 4>(c, s);
-    case 6: return launch_grouped<2, 128, 6, 1, 128, 1, 2>(c, s);
-    case 7: return launch_grouped<1, 128, 8, 0, 32, 1, 2>(c, s);
-    default: return launch_grouped<1, 256, 5, 0, 32, 1, 1, 1, 4>(c, s);
-  }
+  if (variant < 0) variant = choose_grouped_variant(c.p.rows, c.p.groups, c.p.offsets != nullptr, c.p.N, sms);
+  return c.p.offsets ? run_variant<true>(variant, c, s) : run_variant<false>(variant, c, s);
 }
 
 // The checks that the dense and the grouped entry point share.
@@ -855,7 +995,7 @@ extern "C" int b2_nvfp4_grouped_gemm(const void* A, const void* B, const void* S
 }
 
 extern "C" int b2_nvfp4_grouped_gemm_set_variant(int variant) {
-  if (variant < -1 || variant > 8) {
+  if (variant < -1 || variant > 5) {
     b2::set_error("b2_nvfp4_grouped_gemm_set_variant: unknown variant %d", variant);
     return B2_ERR_INVALID_ARGUMENT;
   }

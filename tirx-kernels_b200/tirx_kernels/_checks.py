@@ -105,20 +105,48 @@ def dequantized_matmul_fp32(A_fp4, B_fp4, A_sf, B_sf, alpha: float, *, row_chunk
         torch.set_float32_matmul_precision(precision)
 
 
-def require_tensor(name: str, tensor, dtype, shape) -> None:
-    """ValueError unless `tensor` has this dtype (a torch dtype or its name) and this shape (an int: that many elements)."""
+def tensor_spec(name: str, dtype: str, shape, optional: bool = False) -> tuple:
+    """One argument of an executable: its name, dtype, shape (a tuple, or an int: that many elements), whether it may be None."""
     import torch
 
-    want = getattr(torch, dtype) if isinstance(dtype, str) else dtype
-    if not isinstance(tensor, torch.Tensor):
-        raise ValueError(f"{name} must be a tensor, got {type(tensor).__name__}")
-    if tensor.dtype != want:
-        raise ValueError(f"{name} must be {want}, got {tensor.dtype}")
-    if isinstance(shape, int):
-        if tensor.numel() != shape:
-            raise ValueError(f"{name} must have {shape} elements, got {tensor.numel()}")
-    elif tuple(tensor.shape) != tuple(shape):
-        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(tensor.shape)}")
+    return name, getattr(torch, dtype), shape, optional
+
+
+def require_tensors(specs, tensors) -> int:
+    """ValueError unless every tensor is what its spec says, contiguous and on the current device; returns that device.
+
+    On the launch path of calls that take ten microseconds on the GPU: one pass over plain attributes, and the search for
+    what is wrong only when something is."""
+    import torch
+
+    device = torch.cuda.current_device() if torch.cuda.is_initialized() else -1
+    for spec, t in zip(specs, tensors):
+        if t is None and spec[3]:
+            continue
+        shape = spec[2]
+        if (not isinstance(t, torch.Tensor) or t.dtype is not spec[1] or t.get_device() != device or not t.is_contiguous()
+                or (t.shape != shape if shape.__class__ is tuple else t.numel() != shape) or device < 0):
+            _refuse(spec, t, device)
+    return device
+
+
+def _refuse(spec, t, device: int):
+    import torch
+
+    name, dtype, shape, _ = spec
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{name} must be a tensor, got {type(t).__name__}")
+    if t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+    if isinstance(shape, tuple) and tuple(t.shape) != shape:
+        raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
+    if isinstance(shape, int) and t.numel() != shape:
+        raise ValueError(f"{name} must have {shape} elements, got {t.numel()}")
+    if not t.is_cuda:
+        raise ValueError(f"{name}: all tensors must be CUDA tensors")
+    if not t.is_contiguous():
+        raise ValueError(f"{name}: all tensors must be contiguous")
+    raise ValueError(f"{name} is on {t.device}, but the current device is cuda:{device}")
 
 
 def grouped_sf_numel(rows: int, groups: int, k: int) -> int:

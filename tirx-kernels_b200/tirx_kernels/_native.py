@@ -229,44 +229,15 @@ def nvfp4_gemm_small_m_noalloc(A, B, SFA, SFB, alpha, D, M: int, N: int, K: int)
     )
 
 
-def _require_here(*tensors) -> None:
-    """CUDA, contiguous, and on the current device, whose stream the launch goes to; None is an absent argument."""
+# ---- the feed-forward operators: checked argument by argument in their modules (_checks.require_tensors) ----
+def call(symbol: str, device: int, *args) -> None:
+    """`symbol` with tensors as their addresses (None as null), on the current stream of `device`, the current device."""
     import torch
 
-    present = [t for t in tensors if t is not None]
-    _require_cuda(*present)
-    device = torch.cuda.current_device()
-    for t in present:
-        if t.device.index != device:
-            raise ValueError(f"tensor on {t.device}, but the current device is cuda:{device}")
-
-
-def _ptr_or_null(tensor) -> int | None:
-    return None if tensor is None else tensor.data_ptr()
-
-
-def nvfp4_gemm_epilogue(A, B, SFA, SFB, alpha, bias, residual, D, M: int, N: int, K: int, out_dtype: str,
-                        activation: str = "none") -> None:
-    """D = residual + act(alpha * A B^T + bias); bias and residual may be None."""
-    _require_here(A, B, SFA, SFB, alpha, bias, residual, D)
-    check(
-        lib().b2_nvfp4_gemm_epilogue(_ptr(A), _ptr(B), _ptr(SFA), _ptr(SFB), _ptr(alpha), _ptr_or_null(bias),
-                                     _ptr_or_null(residual), _ptr(D), M, N, K, DTYPE_CODES[out_dtype],
-                                     ACTIVATION_CODES[activation], current_stream_ptr()),
-        "b2_nvfp4_gemm_epilogue",
-    )
-
-
-def nvfp4_grouped_gemm(A, B, SFA, SFB, alpha, offsets, bias, D, rows: int, groups: int, N: int, K: int, out_dtype: str,
-                       activation: str = "none") -> None:
-    """Rows offsets[g]..offsets[g+1] of D = act(alpha[g] * A B[g]^T + bias[g]); bias may be None."""
-    _require_here(A, B, SFA, SFB, alpha, offsets, bias, D)
-    check(
-        lib().b2_nvfp4_grouped_gemm(_ptr(A), _ptr(B), _ptr(SFA), _ptr(SFB), _ptr(alpha), _ptr(offsets),
-                                    _ptr_or_null(bias), _ptr(D), rows, groups, N, K, DTYPE_CODES[out_dtype],
-                                    ACTIVATION_CODES[activation], current_stream_ptr()),
-        "b2_nvfp4_grouped_gemm",
-    )
+    status = getattr(_MAIN or lib(), symbol)(
+        *[a.data_ptr() if isinstance(a, torch.Tensor) else a for a in args], torch._C._cuda_getCurrentRawStream(device))
+    if status != OK:
+        check(status, symbol)
 
 
 def nvfp4_grouped_gemm_set_variant(variant: int) -> None:
@@ -276,64 +247,6 @@ def nvfp4_grouped_gemm_set_variant(variant: int) -> None:
 
 def nvfp4_grouped_gemm_status() -> None:
     check(lib().b2_nvfp4_grouped_gemm_status(current_stream_ptr()), "b2_nvfp4_grouped_gemm_status")
-
-
-def nvfp4_quantize_grouped(inp, index, offsets, out, sf, global_scale, in_rows: int, rows: int, groups: int, k: int,
-                           dtype: str, fuse_silu: bool = False) -> None:
-    """Quantizes row index[r] of `inp` into row r (row r without index), scales in the grouped 128x4 layout."""
-    _require_here(inp, index, offsets, out, sf, global_scale)
-    check(
-        lib().b2_nvfp4_quantize_grouped(_ptr(inp), _ptr_or_null(index), _ptr(offsets), _ptr(out), _ptr(sf),
-                                        _ptr(global_scale), in_rows, rows, groups, k, DTYPE_CODES[dtype],
-                                        int(fuse_silu), current_stream_ptr()),
-        "b2_nvfp4_quantize_grouped",
-    )
-
-
-def moe_plan(ids, offsets, row_token, position, tokens: int, topk: int, experts: int) -> None:
-    _require_here(ids, offsets, row_token, position)
-    check(
-        lib().b2_moe_plan(_ptr(ids), _ptr(offsets), _ptr(row_token), _ptr(position), tokens, topk, experts,
-                          current_stream_ptr()),
-        "b2_moe_plan",
-    )
-
-
-def moe_combine(y, position, weight, residual, out, rows: int, tokens: int, topk: int, n: int, dtype: str) -> None:
-    """out[t] = residual[t] + sum_k weight[t, k] * y[position[t, k]]; residual may be None."""
-    _require_here(y, position, weight, residual, out)
-    check(
-        lib().b2_moe_combine(_ptr(y), _ptr(position), _ptr(weight), _ptr_or_null(residual), _ptr(out), rows, tokens,
-                             topk, n, DTYPE_CODES[dtype], current_stream_ptr()),
-        "b2_moe_combine",
-    )
-
-
-def moe_expert_ffn(x, ids, weight, w1, sf1, alpha1, gs1, w2, sf2, alpha2, gs2, residual, out, workspace, tokens: int,
-                   topk: int, experts: int, hidden: int, inner: int, dtype: str) -> None:
-    _require_here(x, ids, weight, w1, sf1, alpha1, gs1, w2, sf2, alpha2, gs2, residual, out, workspace)
-    check(
-        lib().b2_moe_expert_ffn(_ptr(x), _ptr(ids), _ptr(weight), _ptr(w1), _ptr(sf1), _ptr(alpha1), _ptr(gs1),
-                                _ptr(w2), _ptr(sf2), _ptr(alpha2), _ptr(gs2), _ptr_or_null(residual), _ptr(out),
-                                _ptr(workspace), workspace.numel(), tokens, topk, experts, hidden, inner,
-                                DTYPE_CODES[dtype], current_stream_ptr()),
-        "b2_moe_expert_ffn",
-    )
-
-
-def gated_add_rmsnorm_fp4quant(x, residual, w_post, gate, w_pre, residual_out, y, sf, global_scale, M: int, H: int,
-                               rows_per_gate: int, residual_scale: float, eps: float, dtype: str, quantize: bool,
-                               swizzled: bool) -> None:
-    """w_post and gate may be None; sf and global_scale are None without `quantize`."""
-    _require_here(x, residual, w_post, gate, w_pre, residual_out, y, sf, global_scale)
-    check(
-        lib().b2_gated_add_rmsnorm_fp4quant(_ptr(x), _ptr(residual), _ptr_or_null(w_post), _ptr_or_null(gate),
-                                            _ptr(w_pre), _ptr(residual_out), _ptr(y), _ptr_or_null(sf),
-                                            _ptr_or_null(global_scale), M, H, rows_per_gate, float(residual_scale),
-                                            float(eps), DTYPE_CODES[dtype], int(quantize), int(swizzled),
-                                            current_stream_ptr()),
-        "b2_gated_add_rmsnorm_fp4quant",
-    )
 
 
 def peer_alloc(nbytes: int) -> int:

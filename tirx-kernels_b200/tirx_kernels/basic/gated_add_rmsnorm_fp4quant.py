@@ -29,30 +29,26 @@ def _validate(input_dtype: str, M: int, H: int, rows_per_gate: int) -> None:
 class _Executable:
     def __init__(self, input_dtype: str, M: int, H: int, quantize: bool, swizzled: bool, rows_per_gate: int):
         _validate(input_dtype, M, H, rows_per_gate)
-        self.dtype, self.M, self.H = input_dtype, M, H
-        self.quantize, self.swizzled, self.rows_per_gate = quantize, swizzled, rows_per_gate
+        self.quantize = bool(quantize)
+        spec = _checks.tensor_spec
+        rows = input_dtype, (M, H)
+        self.specs = (
+            spec("x", *rows), spec("residual", *rows), spec("w_post", input_dtype, (H,), True),
+            spec("gate", input_dtype, (_checks.ceil_div(M, rows_per_gate), H), True), spec("w_pre", input_dtype, (H,)),
+            spec("residual_out", *rows), spec("y", "uint8", (M, H // 2)) if quantize else spec("y", *rows),
+        )
+        if quantize:
+            self.specs += (spec("sf", "uint8", _checks.sf_numel(M, H // 16, "128x4" if swizzled else "linear")),
+                           spec("global_scale", "float32", 1))
+        self.sizes = M, H, rows_per_gate
+        self.codes = _native.DTYPE_CODES[input_dtype], int(bool(quantize)), int(bool(swizzled))
 
     def __call__(self, x, residual, w_post, gate, w_pre, residual_out, y, sf, global_scale, residual_scale: float, eps: float) -> None:
-        M, H = self.M, self.H
-        need = _checks.require_tensor
-        need("x", x, self.dtype, (M, H))
-        need("residual", residual, self.dtype, (M, H))
-        if w_post is not None:
-            need("w_post", w_post, self.dtype, (H,))
-        if gate is not None:
-            need("gate", gate, self.dtype, (_checks.ceil_div(M, self.rows_per_gate), H))
-        need("w_pre", w_pre, self.dtype, (H,))
-        need("residual_out", residual_out, self.dtype, (M, H))
-        if self.quantize:
-            need("y", y, "uint8", (M, H // 2))
-            need("sf", sf, "uint8", _checks.sf_numel(M, H // 16, "128x4" if self.swizzled else "linear"))
-            need("global_scale", global_scale, "float32", 1)
-        else:
-            need("y", y, self.dtype, (M, H))
-            if sf is not None or global_scale is not None:
-                raise ValueError("sf and global_scale belong to the quantized form")
-        _native.gated_add_rmsnorm_fp4quant(x, residual, w_post, gate, w_pre, residual_out, y, sf, global_scale, M, H,
-                                           self.rows_per_gate, residual_scale, eps, self.dtype, self.quantize, self.swizzled)
+        if not self.quantize and (sf is not None or global_scale is not None):
+            raise ValueError("sf and global_scale belong to the quantized form")
+        device = _checks.require_tensors(self.specs, (x, residual, w_post, gate, w_pre, residual_out, y, sf, global_scale))
+        _native.call("b2_gated_add_rmsnorm_fp4quant", device, x, residual, w_post, gate, w_pre, residual_out, y, sf, global_scale,
+                     *self.sizes, residual_scale, eps, *self.codes)
 
 
 def get_kernel(input_dtype: str, M: int, H: int, quantize: bool = True, swizzled: bool = True, rows_per_gate: int = 1, **kwargs) -> KernelHandle:

@@ -11,12 +11,35 @@ graph after a first call); ``plan`` and ``combine`` are its first and last step 
 
 from __future__ import annotations
 
+import functools
 from dataclasses import dataclass
 
 from tirx_kernels import _checks, _native, _operator
 from tirx_kernels._protocol import KernelHandle
 
 OPERATOR_META = {"name": "moe_expert_ffn", "category": "basic", "compute_capability": 10}
+
+
+@functools.lru_cache(maxsize=64)
+def _weight_specs(experts: int, inner: int, hidden: int) -> tuple:
+    if not 1 <= experts <= _native.MAX_GROUPS or hidden % 64 or inner % 64 or not hidden or not inner:
+        raise ValueError(f"{experts} experts, hidden={hidden}, inner={inner}: need 1..{_native.MAX_GROUPS} experts, "
+                         "hidden and inner multiples of 64")
+    spec = _checks.tensor_spec
+    scalars = lambda name: spec(name, "float32", (experts,))
+    return (spec("w1", "uint8", (experts, 2 * inner, hidden // 2)),
+            spec("sf1", "uint8", experts * _checks.sf_numel(2 * inner, hidden // 16, "128x4")), scalars("alpha1"), scalars("gs1"),
+            spec("w2", "uint8", (experts, hidden, inner // 2)),
+            spec("sf2", "uint8", experts * _checks.sf_numel(hidden, inner // 16, "128x4")), scalars("alpha2"), scalars("gs2"))
+
+
+@functools.lru_cache(maxsize=256)
+def _call_specs(tokens: int, topk: int, experts: int, hidden: int, inner: int, dtype: str) -> tuple:
+    """(argument specs of expert_ffn, workspace bytes) of a shape."""
+    spec = _checks.tensor_spec
+    rows = dtype, (tokens, hidden)
+    return ((spec("x", *rows), spec("ids", "int32", (tokens, topk)), spec("gates", "float32", (tokens, topk)),
+             spec("residual", *rows, True), spec("out", *rows)), workspace_bytes(tokens, topk, experts, hidden, inner))
 
 
 @dataclass(frozen=True)
@@ -38,19 +61,11 @@ class ExpertWeights:
     gs2: object
 
     def __post_init__(self):
-        need = _checks.require_tensor
         if getattr(self.w1, "ndim", 0) != 3 or getattr(self.w2, "ndim", 0) != 3 or self.w1.shape[1] % 2:
             raise ValueError("w1 and w2 must be [experts, 2 * inner, hidden / 2] and [experts, hidden, inner / 2]")
-        experts, inner, hidden = self.w1.shape[0], self.w1.shape[1] // 2, self.w1.shape[2] * 2
-        if not 1 <= experts <= _native.MAX_GROUPS or hidden % 64 or inner % 64 or not hidden or not inner:
-            raise ValueError(f"{experts} experts, hidden={hidden}, inner={inner}: need 1..{_native.MAX_GROUPS} experts, "
-                             "hidden and inner multiples of 64")
-        need("w1", self.w1, "uint8", (experts, 2 * inner, hidden // 2))
-        need("w2", self.w2, "uint8", (experts, hidden, inner // 2))
-        need("sf1", self.sf1, "uint8", experts * _checks.sf_numel(2 * inner, hidden // 16, "128x4"))
-        need("sf2", self.sf2, "uint8", experts * _checks.sf_numel(hidden, inner // 16, "128x4"))
-        for name in ("alpha1", "gs1", "alpha2", "gs2"):
-            need(name, getattr(self, name), "float32", (experts,))
+        (experts, gate_up, half) = self.w1.shape
+        _checks.require_tensors(_weight_specs(experts, gate_up // 2, half * 2),
+                                (self.w1, self.sf1, self.alpha1, self.gs1, self.w2, self.sf2, self.alpha2, self.gs2))
 
     @property
     def experts(self) -> int:
@@ -74,14 +89,14 @@ def plan(ids, experts: int):
 
     if ids.ndim != 2 or ids.shape[1] < 1:
         raise ValueError(f"ids must be [tokens, topk] with topk >= 1, got {tuple(ids.shape)}")
-    _checks.require_tensor("ids", ids, "int32", tuple(ids.shape))
     if not 1 <= experts <= _native.MAX_GROUPS:
         raise ValueError(f"experts={experts} outside 1..{_native.MAX_GROUPS}")
+    device = _checks.require_tensors((_checks.tensor_spec("ids", "int32", tuple(ids.shape)),), (ids,))
     tokens, topk = ids.shape
     offsets = torch.empty(experts + 1, dtype=torch.int32, device=ids.device)
     row_token = torch.empty(tokens * topk, dtype=torch.int32, device=ids.device)
     position = torch.empty_like(ids)
-    _native.moe_plan(ids, offsets, row_token, position, tokens, topk, experts)
+    _native.call("b2_moe_plan", device, ids, offsets, row_token, position, tokens, topk, experts)
     return offsets, row_token, position
 
 
@@ -95,14 +110,13 @@ def combine(y, position, gates, residual=None, out=None):
     dtype = _operator.dtype_name(y.dtype)
     if n < 8 or n % 8:
         raise ValueError(f"n={n} must be a positive multiple of 8")
-    _checks.require_tensor("position", position, "int32", (tokens, topk))
-    _checks.require_tensor("gates", gates, "float32", (tokens, topk))
-    if residual is not None:
-        _checks.require_tensor("residual", residual, dtype, (tokens, n))
     if out is None:
         out = torch.empty(tokens, n, dtype=y.dtype, device=y.device)
-    _checks.require_tensor("out", out, dtype, (tokens, n))
-    _native.moe_combine(y, position, gates, residual, out, rows, tokens, topk, n, dtype)
+    spec = _checks.tensor_spec
+    device = _checks.require_tensors(
+        (spec("y", dtype, (rows, n)), spec("position", "int32", (tokens, topk)), spec("gates", "float32", (tokens, topk)),
+         spec("residual", dtype, (tokens, n), True), spec("out", dtype, (tokens, n))), (y, position, gates, residual, out))
+    _native.call("b2_moe_combine", device, y, position, gates, residual, out, rows, tokens, topk, n, _native.DTYPE_CODES[dtype])
     return out
 
 
@@ -123,24 +137,23 @@ def expert_ffn(x, ids, gates, weights: ExpertWeights, *, residual=None, out=None
     if getattr(ids, "ndim", 0) != 2 or ids.shape[1] < 1:
         raise ValueError("ids must be [tokens, topk] with topk >= 1")
     tokens, topk = ids.shape
-    experts, hidden, inner = weights.experts, weights.hidden, weights.inner
+    sizes = tokens, topk, *weights.w2.shape[:2], weights.w2.shape[2] * 2
     dtype = _operator.dtype_name(x.dtype)
-    need = _checks.require_tensor
-    need("x", x, dtype, (tokens, hidden))
-    need("ids", ids, "int32", (tokens, topk))
-    need("gates", gates, "float32", (tokens, topk))
-    if residual is not None:
-        need("residual", residual, dtype, (tokens, hidden))
+    specs, size = _call_specs(*sizes, dtype)
     if out is None:
         out = torch.empty_like(x)
-    need("out", out, dtype, (tokens, hidden))
-    size = workspace_bytes(tokens, topk, experts, hidden, inner)
+    device = _checks.require_tensors(specs, (x, ids, gates, residual, out))
     if workspace is None:
         workspace = torch.empty(size, dtype=torch.uint8, device=x.device)
-    elif workspace.dtype != torch.uint8 or workspace.numel() < size:
-        raise ValueError(f"workspace must be uint8 with at least {size} elements, got {workspace.numel()} of {workspace.dtype}")
-    _native.moe_expert_ffn(x, ids, gates, weights.w1, weights.sf1, weights.alpha1, weights.gs1, weights.w2, weights.sf2,
-                           weights.alpha2, weights.gs2, residual, out, workspace, tokens, topk, experts, hidden, inner, dtype)
+    elif (workspace.dtype != torch.uint8 or workspace.numel() < size or workspace.get_device() != device
+          or not workspace.is_contiguous()):
+        raise ValueError(f"workspace must be contiguous uint8 on cuda:{device} with at least {size} elements, got "
+                         f"{workspace.numel()} of {workspace.dtype} on {workspace.device}")
+    if weights.w1.get_device() != device:
+        raise ValueError(f"weights are on {weights.w1.device}, but the current device is cuda:{device}")
+    _native.call("b2_moe_expert_ffn", device, x, ids, gates, weights.w1, weights.sf1, weights.alpha1, weights.gs1, weights.w2,
+                 weights.sf2, weights.alpha2, weights.gs2, residual, out, workspace, workspace.numel(), *sizes,
+                 _native.DTYPE_CODES[dtype])
     return out
 
 
@@ -209,20 +222,21 @@ def _expert(x, weights: ExpertWeights, e: int, dtype: str):
     """Rows through one expert by the package's dense kernels, float64 result."""
     import torch
 
+    from tirx_kernels.basic import nvfp4_gemm_epilogue
+
     rows, hidden, inner = x.shape[0], weights.hidden, weights.inner
     per1, per2 = weights.sf1.numel() // weights.experts, weights.sf2.numel() // weights.experts
     a = torch.empty(rows, hidden // 2, dtype=torch.uint8, device="cuda")
     sfa = torch.empty(_checks.sf_numel(rows, hidden // 16, "128x4"), dtype=torch.uint8, device="cuda")
     y = torch.empty(rows, 2 * inner, dtype=x.dtype, device="cuda")
     _native.nvfp4_quantize(x.contiguous(), a, sfa, weights.gs1[e:e + 1], rows, hidden, dtype, "128x4")
-    _native.nvfp4_gemm_epilogue(a, weights.w1[e], sfa, weights.sf1[e * per1:(e + 1) * per1], weights.alpha1[e:e + 1], None,
-                                None, y, rows, 2 * inner, hidden, dtype)
+    product = lambda N, K: nvfp4_gemm_epilogue.get_kernel(rows, N, K, out_dtype=dtype).config["launcher"]
+    product(2 * inner, hidden)(a, weights.w1[e], sfa, weights.sf1[e * per1:(e + 1) * per1], weights.alpha1[e:e + 1], None, None, y)
     a = torch.empty(rows, inner // 2, dtype=torch.uint8, device="cuda")
     sfa = torch.empty(_checks.sf_numel(rows, inner // 16, "128x4"), dtype=torch.uint8, device="cuda")
     z = torch.empty(rows, hidden, dtype=x.dtype, device="cuda")
     _native.nvfp4_quantize(y, a, sfa, weights.gs2[e:e + 1], rows, inner, dtype, "128x4", fuse_silu=True)
-    _native.nvfp4_gemm_epilogue(a, weights.w2[e], sfa, weights.sf2[e * per2:(e + 1) * per2], weights.alpha2[e:e + 1], None,
-                                None, z, rows, hidden, inner, dtype)
+    product(hidden, inner)(a, weights.w2[e], sfa, weights.sf2[e * per2:(e + 1) * per2], weights.alpha2[e:e + 1], None, None, z)
     return z.double()
 
 

@@ -33,23 +33,18 @@ class _Runner:
 
     def __init__(self, M: int, N: int, K: int, activation: str, out_dtype: str):
         _validate(M, N, K, activation, out_dtype)
-        self.shape, self.activation, self.out_dtype = (M, N, K), activation, out_dtype
-        self.sf_numel = _checks.sf_numel(M, K // 16, "128x4"), _checks.sf_numel(N, K // 16, "128x4")
+        spec = _checks.tensor_spec
+        self.specs = (
+            spec("A", "uint8", (M, K // 2)), spec("B", "uint8", (N, K // 2)),
+            spec("SFA", "uint8", _checks.sf_numel(M, K // 16, "128x4")), spec("SFB", "uint8", _checks.sf_numel(N, K // 16, "128x4")),
+            spec("alpha", "float32", 1), spec("bias", out_dtype, (N,), True), spec("residual", out_dtype, (M, N), True),
+            spec("D", out_dtype, (M, N)),
+        )
+        self.sizes = M, N, K, _native.DTYPE_CODES[out_dtype], _native.ACTIVATION_CODES[activation]
 
     def __call__(self, A, B, SFA, SFB, alpha, bias, residual, D) -> None:
-        M, N, K = self.shape
-        need = _checks.require_tensor
-        need("A", A, "uint8", (M, K // 2))
-        need("B", B, "uint8", (N, K // 2))
-        need("SFA", SFA, "uint8", self.sf_numel[0])
-        need("SFB", SFB, "uint8", self.sf_numel[1])
-        need("alpha", alpha, "float32", 1)
-        if bias is not None:
-            need("bias", bias, self.out_dtype, (N,))
-        if residual is not None:
-            need("residual", residual, self.out_dtype, (M, N))
-        need("D", D, self.out_dtype, (M, N))
-        _native.nvfp4_gemm_epilogue(A, B, SFA, SFB, alpha, bias, residual, D, M, N, K, self.out_dtype, self.activation)
+        device = _checks.require_tensors(self.specs, (A, B, SFA, SFB, alpha, bias, residual, D))
+        _native.call("b2_nvfp4_gemm_epilogue", device, A, B, SFA, SFB, alpha, bias, residual, D, *self.sizes)
 
 
 def get_kernel(M: int, N: int, K: int, activation: str = "none", out_dtype: str = "bfloat16", **kwargs) -> KernelHandle:

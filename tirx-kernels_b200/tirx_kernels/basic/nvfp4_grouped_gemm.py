@@ -30,22 +30,18 @@ def _validate(rows: int, groups: int, N: int, K: int, activation: str, out_dtype
 class _Runner:
     def __init__(self, rows: int, groups: int, N: int, K: int, activation: str, out_dtype: str):
         _validate(rows, groups, N, K, activation, out_dtype)
-        self.shape, self.activation, self.out_dtype = (rows, groups, N, K), activation, out_dtype
-        self.sf_numel = _checks.grouped_sf_numel(rows, groups, K), groups * _checks.sf_numel(N, K // 16, "128x4")
+        spec = _checks.tensor_spec
+        self.specs = (
+            spec("A", "uint8", (rows, K // 2)), spec("B", "uint8", (groups, N, K // 2)),
+            spec("SFA", "uint8", _checks.grouped_sf_numel(rows, groups, K)),
+            spec("SFB", "uint8", groups * _checks.sf_numel(N, K // 16, "128x4")), spec("alpha", "float32", (groups,)),
+            spec("offsets", "int32", (groups + 1,)), spec("bias", out_dtype, (groups, N), True), spec("D", out_dtype, (rows, N)),
+        )
+        self.sizes = rows, groups, N, K, _native.DTYPE_CODES[out_dtype], _native.ACTIVATION_CODES[activation]
 
     def __call__(self, A, B, SFA, SFB, alpha, offsets, bias, D) -> None:
-        rows, groups, N, K = self.shape
-        need = _checks.require_tensor
-        need("A", A, "uint8", (rows, K // 2))
-        need("B", B, "uint8", (groups, N, K // 2))
-        need("SFA", SFA, "uint8", self.sf_numel[0])
-        need("SFB", SFB, "uint8", self.sf_numel[1])
-        need("alpha", alpha, "float32", (groups,))
-        need("offsets", offsets, "int32", (groups + 1,))
-        if bias is not None:
-            need("bias", bias, self.out_dtype, (groups, N))
-        need("D", D, self.out_dtype, (rows, N))
-        _native.nvfp4_grouped_gemm(A, B, SFA, SFB, alpha, offsets, bias, D, rows, groups, N, K, self.out_dtype, self.activation)
+        device = _checks.require_tensors(self.specs, (A, B, SFA, SFB, alpha, offsets, bias, D))
+        _native.call("b2_nvfp4_grouped_gemm", device, A, B, SFA, SFB, alpha, offsets, bias, D, *self.sizes)
 
 
 def get_kernel(rows: int, groups: int, N: int, K: int, activation: str = "none", out_dtype: str = "bfloat16", **kwargs) -> KernelHandle:
@@ -69,6 +65,8 @@ def prepare_data(rows: int, groups: int, N: int, K: int, out_dtype: str = "bfloa
     """Seeded (A, B, SFA, SFB, alpha, offsets, bias); `sizes` rows per group, else uneven groups, some of them empty."""
     import torch
 
+    from tirx_kernels.basic import nvfp4_quantize_grouped
+
     generator = torch.Generator().manual_seed(1)
     draw = lambda *shape: torch.randn(*shape, generator=generator)
     if sizes is None:
@@ -81,7 +79,7 @@ def prepare_data(rows: int, groups: int, N: int, K: int, out_dtype: str = "bfloa
     gs = (2688.0 / (5.0 + torch.rand(groups, generator=generator))).cuda()
     A = torch.zeros(rows, K // 2, dtype=torch.uint8, device="cuda")
     SFA = torch.full((_checks.grouped_sf_numel(rows, groups, K),), 0xFF, dtype=torch.uint8, device="cuda")  # NaN where no row is
-    _native.nvfp4_quantize_grouped(x, None, offsets, A, SFA, gs, rows, rows, groups, K, "bfloat16")
+    nvfp4_quantize_grouped.get_kernel("bfloat16", rows, rows, groups, K).config["launcher"](x, None, offsets, A, SFA, gs)
     B, SFB, gs_b = quantize_weights((0.02 * draw(groups, N, K)).to(torch.bfloat16).cuda())
     return A, B, SFA, SFB, 1.0 / (gs * gs_b), offsets, draw(groups, N).to(_operator.torch_dtype(out_dtype)).cuda() if bias else None
 

@@ -29,19 +29,17 @@ def _validate(dtype: str, in_rows: int, rows: int, groups: int, k: int) -> None:
 class _Executable:
     def __init__(self, dtype: str, in_rows: int, rows: int, groups: int, k: int, fuse_silu: bool):
         _validate(dtype, in_rows, rows, groups, k)
-        self.dtype, self.in_rows, self.rows, self.groups, self.k, self.fuse_silu = dtype, in_rows, rows, groups, k, fuse_silu
+        spec = _checks.tensor_spec
+        self.specs = (
+            spec("x", dtype, (in_rows, k * (2 if fuse_silu else 1))), spec("index", "int32", (rows,), True),
+            spec("offsets", "int32", (groups + 1,)), spec("out", "uint8", (rows, k // 2)),
+            spec("sf", "uint8", _checks.grouped_sf_numel(rows, groups, k)), spec("global_scale", "float32", (groups,)),
+        )
+        self.sizes = in_rows, rows, groups, k, _native.DTYPE_CODES[dtype], int(fuse_silu)
 
     def __call__(self, x, index, offsets, out, sf, global_scale) -> None:
-        need = _checks.require_tensor
-        need("x", x, self.dtype, (self.in_rows, self.k * (2 if self.fuse_silu else 1)))
-        if index is not None:
-            need("index", index, "int32", (self.rows,))
-        need("offsets", offsets, "int32", (self.groups + 1,))
-        need("out", out, "uint8", (self.rows, self.k // 2))
-        need("sf", sf, "uint8", _checks.grouped_sf_numel(self.rows, self.groups, self.k))
-        need("global_scale", global_scale, "float32", (self.groups,))
-        _native.nvfp4_quantize_grouped(x, index, offsets, out, sf, global_scale, self.in_rows, self.rows, self.groups,
-                                       self.k, self.dtype, self.fuse_silu)
+        device = _checks.require_tensors(self.specs, (x, index, offsets, out, sf, global_scale))
+        _native.call("b2_nvfp4_quantize_grouped", device, x, index, offsets, out, sf, global_scale, *self.sizes)
 
 
 def get_kernel(dtype: str, in_rows: int, rows: int, groups: int, k: int, fuse_silu: bool = False, **kwargs) -> KernelHandle:
