@@ -291,9 +291,20 @@ int b2_nvfp4_grouped_gemm(const void* A, const void* B, const void* SFA, const v
                           const int32_t* offsets_dev, const void* bias, void* D, int rows, int groups, int N, int K,
                           int out_dtype, int activation, void* stream);
 
-/* Kernel variant of the following calls of the two products (-1: automatic): tiles of 0 32 x 64 (dense, two MMA warps),
+/*
+ * The first product of a gated feed-forward with the second one's quantizer in its epilogue: B is [groups, 2 * inner, K/2],
+ * gate rows in front of up rows, and SiLU(gate) * up leaves as packed E2M1 [rows, inner/2] with its scales in the grouped
+ * 128x4 layout (b2_nvfp4_grouped_sf_bytes(rows, groups, inner), 16-byte aligned), quantized with gs_dev[group].
+ * The bytes are those of b2_nvfp4_grouped_gemm to `dtype` followed by b2_nvfp4_quantize_grouped with fuse_silu; the
+ * 16-bit product never reaches memory.  inner % 128 == 0; all else as b2_nvfp4_grouped_gemm.
+ */
+int b2_nvfp4_grouped_gemm_gated(const void* A, const void* B, const void* SFA, const void* SFB, const float* alpha_dev,
+                                const int32_t* offsets_dev, const float* gs_dev, void* out, void* sf, int rows,
+                                int groups, int inner, int K, int dtype, void* stream);
+
+/* Kernel variant of the following calls of the products (-1: automatic): tiles of 0 32 x 64 (dense, two MMA warps),
  * 1 32 x 128, 2 128 x 64 (dense, two MMA warps), 3 128 x 128, 4 256 x 256 (a CTA pair), 5 256 x 128 (a CTA pair).  Every
- * variant takes every shape (grouped calls run 1 for 0 and 3 for 2). */
+ * variant takes every shape (grouped calls run 1 for 0 and 3 for 2, gated ones also 4 for 5). */
 int b2_nvfp4_grouped_gemm_set_variant(int variant);
 
 /* Reads and clears the status words of the two products on the current device, as b2_nvfp4_gemm_status. */
@@ -323,6 +334,16 @@ int b2_moe_plan(const int32_t* ids_dev, int32_t* offsets_dev, int32_t* row_token
                 int topk, int experts, void* stream);
 
 /*
+ * Plan and quantizer in one call: every row of x [tokens, k] is quantized for each of its experts, with that expert's
+ * encode scale gs_dev[experts], into the row that b2_moe_plan gives the assignment; out, sf as b2_nvfp4_quantize_grouped
+ * with tokens * topk rows.  Writes offsets and position as b2_moe_plan; row_token_dev is scratch of tokens * topk words
+ * (its contents are not specified).  topk <= 32.
+ */
+int b2_moe_dispatch(const void* x, const int32_t* ids_dev, const float* gs_dev, int32_t* offsets_dev,
+                    int32_t* row_token_dev, int32_t* position_dev, void* out, void* sf, int tokens, int topk,
+                    int experts, int k, int dtype, void* stream);
+
+/*
  * out[t] = residual[t] + sum over k of weight[t,k] * y[position[t,k]], in order of k, fp32 with one rounding.
  *   y [rows, n], residual [tokens, n] or NULL (may be out), out [tokens, n], all of dtype; position int32, weight fp32
  *   [tokens, topk].  Positions outside [0, rows) add nothing.  n % 8 == 0, 16-byte aligned tensors.
@@ -333,12 +354,13 @@ int b2_moe_combine(const void* y, const int32_t* position_dev, const float* weig
 /*
  * Routed feed-forward: plan, quantize x per expert, product with W1 (uint8 [experts, 2 * inner, hidden/2], gate rows
  * in front of up rows), SiLU(gate) * up quantized per expert, product with W2 (uint8 [experts, hidden, inner/2]),
- * weighted sum per token.  Six launches on `stream`, each of the entry points above.
+ * weighted sum per token: the entry points above, four launches on `stream` (one more for over 512 assignments, one more
+ * when inner is no multiple of 128).
  *   x, residual (or NULL), out [tokens, hidden] of dtype; alpha1, gs1, alpha2, gs2 fp32 [experts]: gs the encode scale of
  *   the activations, alpha 1 / (gs * the weight's encode scale)
  *   workspace  b2_moe_expert_ffn_workspace_bytes(...) bytes, 256-byte aligned; its contents need not be kept between
  *              calls, and calls that may overlap (other streams, graphs replayed at once) need one each
- * hidden and inner are multiples of 64.
+ * hidden and inner are multiples of 64, topk <= 32.
  */
 int b2_moe_expert_ffn(const void* x, const int32_t* ids_dev, const float* weight_dev, const void* W1, const void* SF1,
                       const float* alpha1_dev, const float* gs1_dev, const void* W2, const void* SF2,

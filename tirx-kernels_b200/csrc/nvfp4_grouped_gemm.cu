@@ -29,6 +29,7 @@
 #include <atomic>
 
 #include "nvfp4_tile.cuh"
+#include "quant_block.cuh"
 
 namespace b2 {
 namespace {
@@ -51,11 +52,19 @@ struct GroupedParams {
   int act;                  // B2_ACT_*
   int fp16;                 // 16-bit type of bias, residual and D
   uint64_t wait_budget_ns;
+  // kGated: the weight is [gate rows | up rows] of N / 2 each, and SiLU(gate) * up leaves quantized
+  const float* gs;          // [groups] encode scale of the output
+  uint8_t* out4;            // [rows, N / 4] packed E2M1
+  uint8_t* sf_out;          // grouped 128 x 4 scale tiles
 };
 
-template <int CG, int BN, int STAGES, int TMA_OUT, int AM>
-struct GroupedLayout : SmemLayout<CG, BN, STAGES, TMA_OUT, AM> {
-  using Base = SmemLayout<CG, BN, STAGES, TMA_OUT, AM>;
+// What a kernel multiplies and how it ends: one group known to the host; groups; groups, with SiLU(gate) * up quantized.
+enum Mode { kDense, kGrouped, kGated };
+
+// A gated tile of a single CTA takes its columns from two places of the weight, half from each: two scale chunks.
+template <Mode MODE, int CG, int BN, int STAGES, int TMA_OUT, int AM>
+struct GroupedLayout : SmemLayout<CG, BN, STAGES, TMA_OUT, AM, MODE == kGated ? 2 : 0> {
+  using Base = SmemLayout<CG, BN, STAGES, TMA_OUT, AM, MODE == kGated ? 2 : 0>;
   static constexpr int kTable = Base::kRingBytes + Base::kBarrierBytes;
   static constexpr int kAll = kTable + kTableBytes + 1024;  // + alignment slack
   static_assert(kAll <= 227 * 1024, "shared memory budget");
@@ -68,10 +77,10 @@ struct Tile {
 
 // Work item t -> its tile.  starts[g] is the number of row tiles in front of group g; among groups without rows,
 // which share a start, bisection ends at the last one, the one that has the tile.
-template <bool GROUPED>
+template <Mode MODE>
 __device__ __forceinline__ Tile find_tile(const GroupedParams& p, const int* starts, const int* rows, int t) {
   Tile r;
-  if constexpr (!GROUPED) {
+  if constexpr (MODE == kDense) {
     r.group = 0;
     r.first = 0;
     r.last = p.rows;
@@ -176,6 +185,9 @@ __device__ __forceinline__ void pack(uint32_t* v) {
   for (int i = 0; i < N / 2; ++i) v[i] = pack_from_f32<Tag>(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
 }
 
+__device__ __forceinline__ void lds64(uint32_t addr, uint32_t* r) {
+  asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(addr));
+}
 __device__ __forceinline__ uint4 lds128_vec(uint32_t addr) {
   uint32_t r[4];
   lds128(addr, r);
@@ -207,6 +219,37 @@ __device__ __forceinline__ void take_registers() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS));
 }
 
+// 32 gate and 32 up columns of one row -> SiLU(gate) * up in NVFP4: two blocks, with the bits that the 16-bit product
+// followed by the quantizer's fuse_silu gives (the same roundings: product to 16 bits, SiLU * up to 16 bits).
+template <typename Tag>
+__device__ __forceinline__ void gated_blocks(const GroupedParams& p, const uint32_t* v, float alpha, int group, int row,
+                                             int64_t sf_row, int col) {
+  const float gs = __ldg(p.gs + group);
+  const float rcp_gs = rcp_approx_ftz(gs), rcp6 = rcp_approx_ftz(6.0f);
+  uint32_t codes = 0;
+  uint2 packed[2];
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t* g = v + 16 * b + 2 * i;
+      const uint32_t gate = pack_from_f32<Tag>(__uint_as_float(g[0]) * alpha, __uint_as_float(g[1]) * alpha);
+      const uint32_t up = pack_from_f32<Tag>(__uint_as_float(g[32]) * alpha, __uint_as_float(g[33]) * alpha);
+      w[i] = silu_and_mul_pair<Tag>(gate, up);
+    }
+    uint32_t sf_byte;
+    quantize_block<Tag>(w, gs, rcp_gs, rcp6, sf_byte, packed[b]);
+    codes |= sf_byte << (8 * b);
+  }
+  const int cols = p.N / 32;  // scale blocks of a row
+  *reinterpret_cast<uint16_t*>(p.sf_out + (col / 16 & 3) + static_cast<int64_t>(col / 64) * 512 + (sf_row & 31) * 16 +
+                               ((sf_row & 127) >> 5) * 4 + (sf_row >> 7) * (128 * static_cast<int64_t>(cols))) =
+      static_cast<uint16_t>(codes);
+  *reinterpret_cast<uint4*>(p.out4 + static_cast<int64_t>(row) * (p.N / 4) + col / 2) =
+      make_uint4(packed[0].x, packed[0].y, packed[1].x, packed[1].y);
+}
+
 // CG: CTAs of a tile (1 or 2).  BN: its columns.  AM: rows of A that one CTA loads and multiplies (the MMA reads 128;
 // what follows a shorter box in the stage only reaches accumulator rows that nobody reads).  MMAS: MMA-issuing warps
 // with an accumulator each, for a single tile per CTA (issuing is the limit there).  NACC: accumulators in turn, for many tiles.
@@ -216,13 +259,13 @@ constexpr int group_threads(int sets, int parts) { return 32 * (4 + 4 * sets + 4
 constexpr int kRegsLaunch = 80, kRegsIssue = 56, kRegsScale = 40, kRegsEpilogue = 96;
 static_assert(kRegsIssue + kRegsScale + 4 * kRegsEpilogue <= 6 * kRegsLaunch, "no warpgroup waits for registers that nobody gives");
 
-template <bool GROUPED, int CG, int BN, int STAGES, int TMA_OUT, int AM, int MMAS, int NACC, int SETS, int PARTS>
+template <Mode MODE, int CG, int BN, int STAGES, int TMA_OUT, int AM, int MMAS, int NACC, int SETS, int PARTS>
 __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
     nvfp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                               const __grid_constant__ CUtensorMap map_sfa, const __grid_constant__ CUtensorMap map_sfb,
                               const __grid_constant__ CUtensorMap map_d, const __grid_constant__ CUtensorMap map_r,
                               const __grid_constant__ GroupedParams p) {
-  using L = GroupedLayout<CG, BN, STAGES, TMA_OUT, AM>;
+  using L = GroupedLayout<MODE, CG, BN, STAGES, TMA_OUT, AM>;
   static_assert(MMAS == 1 || (CG == 1 && TMA_OUT == 0), "the second MMA warp exists for single-CTA tiles");
   static_assert(CG == 1 || AM == kBlockM, "pairs load all rows");
   constexpr int kBM = AM * CG;                // rows of a tile
@@ -296,7 +339,7 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
   // Dependent launch as in nvfp4_gemm.cu: nothing in front of this wait touches global memory.
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if constexpr (GROUPED) {
+  if constexpr (MODE != kDense) {
     if (warp == kGWarpMma2) {
       int tiles = 0;  // row tiles in front of the 32 groups of this step
       for (int g0 = 0; g0 < p.groups; g0 += 32) {
@@ -330,7 +373,7 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
   // What the issuing warps compute from shared memory is made uniform by a shuffle, or the compiler would keep their
   // loops' state out of uniform registers (nvfp4_gemm.cu).
   auto uniform = [](int v) { return kWarpWide ? __shfl_sync(0xffffffffu, v, 0) : v; };
-  const int num_tiles = GROUPED ? uniform(starts[p.groups]) * p.tiles_n : p.tiles_m * p.tiles_n;
+  const int num_tiles = MODE != kDense ? uniform(starts[p.groups]) * p.tiles_n : p.tiles_m * p.tiles_n;
   const int k_slabs = p.k_slabs;
 
   // The waits of the issuing roles: of the whole warp with one outcome, or of lane 0.
@@ -357,9 +400,11 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
       uint32_t phase = 0;
       bool alive = true;
       for (int t = unit; t < num_tiles && alive; t += num_units) {
-        const Tile tile = find_tile<GROUPED>(p, starts, group_rows, t);
+        const Tile tile = find_tile<MODE>(p, starts, group_rows, t);
         const int row_a = uniform(tile.first + tile.tm * kBM) + static_cast<int>(rank) * kBlockM;
-        const int row_b = uniform(tile.group * p.N + tile.tn * BN) + static_cast<int>(rank) * L::kBRows;
+        // Gated: the first half of the tile's columns are gates, the second (the pair's second CTA's) the matching ups.
+        const int row_b = MODE == kGated ? uniform(tile.group * p.N + tile.tn * (BN / 2)) + static_cast<int>(rank) * (p.N / 2)
+                                         : uniform(tile.group * p.N + tile.tn * BN) + static_cast<int>(rank) * L::kBRows;
         for (int ks = 0; ks < k_slabs; ++ks) {
           if (!role_wait(empty_bar(stage), phase ^ 1u, 1u)) { alive = false; break; }
           const uint32_t sbase = smem_base + stage * L::kStageBytes;
@@ -369,6 +414,8 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
             if (leader) mbar_expect_tx(full_bar(stage), kOperandTx);
             tma_load_2d<CG>(sbase, &map_a, ks * 128, row_a, op_bar);
             tma_load_2d<CG>(sbase + L::kABytes, &map_b, ks * 128, row_b, op_bar);
+            if constexpr (MODE == kGated && CG == 1)
+              tma_load_2d<CG>(sbase + L::kABytes + L::kBBytes / 2, &map_b, ks * 128, row_b + p.N / 2, op_bar);
           }
           if constexpr (kWarpWide) __syncwarp();
           if (++stage == STAGES) { stage = 0; phase ^= 1u; }
@@ -383,9 +430,9 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
       uint32_t phase = 0;
       bool alive = true;
       for (int t = unit; t < num_tiles && alive; t += num_units) {
-        const Tile tile = find_tile<GROUPED>(p, starts, group_rows, t);
+        const Tile tile = find_tile<MODE>(p, starts, group_rows, t);
         const int sfa_tile = uniform((tile.first >> 7) + tile.group + ((tile.tm * kBM) >> 7)) + static_cast<int>(rank);
-        const int sfb_tile = uniform(tile.group * sfb_tiles + (tile.tn * BN) / 128);
+        const int sfb_tile = uniform(tile.group * sfb_tiles + (tile.tn * (MODE == kGated ? BN / 2 : BN)) / 128);
         for (int ks = 0; ks < k_slabs; ++ks) {
           if (!role_wait(empty_bar(stage), phase ^ 1u, 1u)) { alive = false; break; }
           const uint32_t sf_smem = smem_base + stage * L::kStageBytes + L::kABytes + L::kBBytes;
@@ -393,6 +440,8 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
             mbar_expect_tx(sfload_bar(stage), kScaleTx);
             tma_load_3d<1>(sf_smem, &map_sfa, 0, ks * 4, sfa_tile, sfload_bar(stage));
             tma_load_3d<1>(sf_smem + L::kSfaBytes, &map_sfb, 0, ks * 4, sfb_tile, sfload_bar(stage));
+            if constexpr (MODE == kGated)
+              tma_load_3d<1>(sf_smem + L::kSfaBytes + 2048, &map_sfb, 0, ks * 4, sfb_tile + p.N / 256, sfload_bar(stage));
           }
           if constexpr (kWarpWide) __syncwarp();
           if (++stage == STAGES) { stage = 0; phase ^= 1u; }
@@ -413,7 +462,7 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
         tc_fence_after();
         // A 64-wide tile uses half of a 128-row scale chunk of B: the upper half starts two columns in.
         uint32_t sfb_half = 0;
-        if constexpr (BN == 64) sfb_half = static_cast<uint32_t>(find_tile<GROUPED>(p, starts, group_rows, t).tn & 1) * 2u;
+        if constexpr (BN == 64) sfb_half = static_cast<uint32_t>(find_tile<MODE>(p, starts, group_rows, t).tn & 1) * 2u;
         const uint32_t acc_tmem = tmem_base + static_cast<uint32_t>((acc * MMAS + me) * BN);
         int stage = (slab0 + me) % STAGES;
         uint32_t phase = static_cast<uint32_t>((slab0 + me) / STAGES) & 1u;
@@ -465,12 +514,16 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
     const int quarter = warp & 3;
     const int set = (warp - kGWarpScale0) >> 2;
     const int total_slabs = unit < num_tiles ? ((num_tiles - unit + num_units - 1) / num_units) * k_slabs : 0;
-    int tile_slabs = 0, t = unit;  // slabs left of the current tile, the next tile (AM == 32 only)
+    constexpr bool kHalves = MODE == kGated && CG == 1;  // 64 gate and 64 up columns, each half of a scale chunk
+    int tile_slabs = 0, t = unit;  // slabs left of the current tile, the next tile (AM == 32 and kHalves only)
     int part = 0;                  // the 32-row quarter of the scale tile that this tile's rows have
+    uint32_t half_bytes = 0;       // the 64-row half of the scale chunks that this tile's columns have
     for (int n = 0; n < total_slabs; ++n) {
-      if constexpr (AM == 32) {
+      if constexpr (AM == 32 || kHalves) {
         if (tile_slabs == 0) {
-          part = find_tile<GROUPED>(p, starts, group_rows, t).tm & 3;
+          const Tile tile = find_tile<MODE>(p, starts, group_rows, t);
+          part = tile.tm & 3;
+          half_bytes = static_cast<uint32_t>(tile.tn & 1) * 8u;
           t += num_units;
           tile_slabs = k_slabs;
         }
@@ -487,6 +540,11 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
       auto load_b = [&](int c, uint32_t* b) {  // words 16 c .. 16 c + 15 of [kb][chunk][4]
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
+          if constexpr (kHalves) {  // [kb][gate 2, up 2]
+            lds64(sfb_smem + i * 512 + half_bytes, b + 4 * i);
+            lds64(sfb_smem + 2048 + i * 512 + half_bytes, b + 4 * i + 2);
+            continue;
+          }
           const int word = 4 * c + i;
           lds128(sfb_smem + ((word % L::kChunks) * 4 + word / L::kChunks) * 512, b + 4 * i);
         }
@@ -542,13 +600,13 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int t = unit; t < num_tiles; t += num_units) {
-      const Tile tile = find_tile<GROUPED>(p, starts, group_rows, t);
+      const Tile tile = find_tile<MODE>(p, starts, group_rows, t);
       const float alpha = __ldg(p.alpha + tile.group);
       const int in_tile = static_cast<int>(rank) * kBlockM + quarter * 32;  // first row of this warp in the tile
       const int row0 = tile.first + tile.tm * kBM + in_tile;
       const int row = row0 + lane;
       const int col0 = tile.tn * BN + part * kCols;
-      const bool any = in_tile < kBM && row0 < tile.last && col0 < p.N;  // the same in the whole warp
+      const bool any = in_tile < kBM && row0 < tile.last && (MODE == kGated || col0 < p.N);  // the same in the whole warp
       const bool mine = any && row < tile.last;
       const int64_t at = static_cast<int64_t>(row) * p.N + col0;
       const uint16_t* bias = p.bias ? p.bias + static_cast<int64_t>(tile.group) * p.N + col0 : nullptr;
@@ -583,7 +641,8 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
                                   static_cast<uint32_t>(acc * MMAS * BN + part * kCols);
 #pragma unroll
         for (int c0 = 0; c0 < kCols; c0 += 32)
-          tmem_ld_32x32(acc_tmem + c0, *reinterpret_cast<uint32_t(*)[32]>(v + c0));
+          tmem_ld_32x32(MODE == kGated ? acc_tmem - part * 32 + c0 / 32 * (BN / 2) : acc_tmem + c0,
+                        *reinterpret_cast<uint32_t(*)[32]>(v + c0));
         if (MMAS == 1 || !two) tmem_ld_wait();
         if constexpr (MMAS == 2) {
           if (two) {
@@ -606,6 +665,14 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
       }
       if (++acc == NACC) { acc = 0; acc_phase ^= 1u; }
       if (!any) continue;
+      if constexpr (MODE == kGated) {
+        if (mine) {
+          const int64_t sf_row = (static_cast<int64_t>(tile.first >> 7) + tile.group) * 128 + row - tile.first;
+          if (p.fp16) gated_blocks<F16Tag>(p, v, alpha, tile.group, row, sf_row, tile.tn * (BN / 2) + part * 32);
+          else gated_blocks<BF16Tag>(p, v, alpha, tile.group, row, sf_row, tile.tn * (BN / 2) + part * 32);
+        }
+        continue;
+      }
       // The TMA clips rows behind the last row and columns behind N, but knows nothing of groups.
       const bool by_tma = TMA_OUT > 0 && (row0 + 32 <= tile.last || tile.last == p.rows);
       const int left = p.N - col0;
@@ -741,17 +808,18 @@ int encode_store_map(CUtensorMap* map, void* base, int rows, int N) {
   return B2_OK;
 }
 
-template <bool GROUPED, int CG, int BN, int STAGES, int TMA_OUT, int AM, int MMAS, int NACC, int SETS = 2, int PARTS = 2>
+template <Mode MODE, int CG, int BN, int STAGES, int TMA_OUT, int AM, int MMAS, int NACC, int SETS = 2, int PARTS = 2>
 int launch_grouped(const GroupedCall& c, cudaStream_t stream) {
-  using L = GroupedLayout<CG, BN, STAGES, TMA_OUT, AM>;
+  using L = GroupedLayout<MODE, CG, BN, STAGES, TMA_OUT, AM>;
   constexpr int kBM = AM * CG;
-  auto kernel = nvfp4_grouped_gemm_kernel<GROUPED, CG, BN, STAGES, TMA_OUT, AM, MMAS, NACC, SETS, PARTS>;
+  auto kernel = nvfp4_grouped_gemm_kernel<MODE, CG, BN, STAGES, TMA_OUT, AM, MMAS, NACC, SETS, PARTS>;
   GroupedParams p = c.p;
   CUtensorMap map_a, map_b, map_sfa, map_sfb, map_d = {}, map_r = {};
   if (int rc = encode_operand_map(&map_a, c.A, p.rows, c.K, AM)) return rc;
-  if (int rc = encode_operand_map(&map_b, c.B, p.groups * p.N, c.K, L::kBRows)) return rc;
+  if (int rc = encode_operand_map(&map_b, c.B, p.groups * p.N, c.K, MODE == kGated ? BN / 2 : L::kBRows)) return rc;
   if (int rc = encode_scale_map(&map_sfa, c.SFA, c.sfa_tiles * 128, c.K, 1)) return rc;
-  if (int rc = encode_scale_map(&map_sfb, c.SFB, p.groups * ((p.N + 127) / 128) * 128, c.K, L::kChunks)) return rc;
+  if (int rc = encode_scale_map(&map_sfb, c.SFB, p.groups * ((p.N + 127) / 128) * 128, c.K, MODE == kGated ? 1 : L::kChunks))
+    return rc;
   if (TMA_OUT > 0) {
     if (int rc = encode_store_map(&map_d, p.D, p.rows, p.N)) return rc;
     if (p.residual)
@@ -759,12 +827,12 @@ int launch_grouped(const GroupedCall& c, cudaStream_t stream) {
   }
   p.k_slabs = (c.K + kBlockK - 1) / kBlockK;
   p.tiles_m = (p.rows + kBM - 1) / kBM;
-  p.tiles_n = (p.N + BN - 1) / BN;
+  p.tiles_n = (p.N + BN - 1) / BN;  // gated: BN / 2 gates and BN / 2 ups a tile, the same number
   p.group_n = 8;
   const int sms = device_sm_count();
   if (sms <= 0) return B2_ERR_CUDA;
   // The most row tiles that the groups can have; for one group that is their number.
-  const int64_t tiles_m = GROUPED ? p.rows / kBM + static_cast<int64_t>(p.groups < p.rows ? p.groups : p.rows)
+  const int64_t tiles_m = MODE != kDense ? p.rows / kBM + static_cast<int64_t>(p.groups < p.rows ? p.groups : p.rows)
                                   : p.tiles_m;
   const int64_t tiles = tiles_m * p.tiles_n;
   if (tiles > 0x3fffffff) {
@@ -867,18 +935,35 @@ int choose_grouped_variant(int rows, int groups, bool grouped, int N, int sms) {
   return (2 * (rows / 256) + groups) * n256 <= 2 * sms ? 5 : 4;
 }
 
-// The two-MMA-warp kernels are for one tile per CTA, which only a dense product knows to have.
-template <bool GROUPED>
-int run_variant(int variant, const GroupedCall& c, cudaStream_t s) {
+// The two-MMA-warp kernels are for one tile per CTA, which only a dense product knows to have.  Gated, a stage of the
+// 128 x 128 tiles holds one more scale chunk (five stages for six), and pairs take 256 columns: 128 gates, 128 ups.
+int run_dense(int variant, const GroupedCall& c, cudaStream_t s) {
+  switch (variant) {
+    case 0: return launch_grouped<kDense, 1, 64, 11, 0, 32, 2, 1>(c, s);
+    case 1: return launch_grouped<kDense, 1, 128, 8, 0, 32, 1, 2>(c, s);
+    case 2: return launch_grouped<kDense, 1, 64, 7, 0, 128, 2, 1>(c, s);
+    case 3: return launch_grouped<kDense, 1, 128, 6, 0, 128, 1, 2>(c, s);
+    case 4: return launch_grouped<kDense, 2, 256, 5, 1, 128, 1, 1, 1, 4>(c, s);
+    default: return launch_grouped<kDense, 2, 128, 6, 1, 128, 1, 2>(c, s);
+  }
+}
+int run_groups(int variant, const GroupedCall& c, cudaStream_t s) {
   switch (variant) {
     case 0:
-      if constexpr (!GROUPED) return launch_grouped<false, 1, 64, 11, 0, 32, 2, 1>(c, s);
-    case 1: return launch_grouped<GROUPED, 1, 128, 8, 0, 32, 1, 2>(c, s);
+    case 1: return launch_grouped<kGrouped, 1, 128, 8, 0, 32, 1, 2>(c, s);
     case 2:
-      if constexpr (!GROUPED) return launch_grouped<false, 1, 64, 7, 0, 128, 2, 1>(c, s);
-    case 3: return launch_grouped<GROUPED, 1, 128, 6, 0, 128, 1, 2>(c, s);
-    case 4: return launch_grouped<GROUPED, 2, 256, 5, 1, 128, 1, 1, 1, 4>(c, s);
-    default: return launch_grouped<GROUPED, 2, 128, 6, 1, 128, 1, 2>(c, s);
+    case 3: return launch_grouped<kGrouped, 1, 128, 6, 0, 128, 1, 2>(c, s);
+    case 4: return launch_grouped<kGrouped, 2, 256, 5, 1, 128, 1, 1, 1, 4>(c, s);
+    default: return launch_grouped<kGrouped, 2, 128, 6, 1, 128, 1, 2>(c, s);
+  }
+}
+int run_gated(int variant, const GroupedCall& c, cudaStream_t s) {
+  switch (variant) {
+    case 0:
+    case 1: return launch_grouped<kGated, 1, 128, 8, 0, 32, 1, 2>(c, s);
+    case 2:
+    case 3: return launch_grouped<kGated, 1, 128, 5, 0, 128, 1, 2>(c, s);
+    default: return launch_grouped<kGated, 2, 256, 5, 0, 128, 1, 1, 1, 4>(c, s);
   }
 }
 
@@ -887,7 +972,8 @@ int run_grouped(const GroupedCall& c, cudaStream_t s) {
   if (sms <= 0) return B2_ERR_CUDA;
   int variant = g_grouped_variant.load(std::memory_order_relaxed);
   if (variant < 0) variant = choose_grouped_variant(c.p.rows, c.p.groups, c.p.offsets != nullptr, c.p.N, sms);
-  return c.p.offsets ? run_variant<true>(variant, c, s) : run_variant<false>(variant, c, s);
+  if (c.p.out4) return run_gated(variant, c, s);
+  return c.p.offsets ? run_groups(variant, c, s) : run_dense(variant, c, s);
 }
 
 // The checks that the dense and the grouped entry point share.
@@ -912,14 +998,14 @@ int check_product(const GroupedCall& c, int out_dtype) {
     return B2_ERR_INVALID_ARGUMENT;
   }
   if (p.rows == 0) return B2_OK;
-  if (!c.A || !c.B || !c.SFA || !c.SFB || !p.alpha || !p.D) {
+  if (!c.A || !c.B || !c.SFA || !c.SFB || !p.alpha || (!p.D && !p.out4)) {
     set_error("%s: null pointer argument", c.who);
     return B2_ERR_INVALID_ARGUMENT;
   }
   const uintptr_t all = reinterpret_cast<uintptr_t>(c.A) | reinterpret_cast<uintptr_t>(c.B) |
                         reinterpret_cast<uintptr_t>(c.SFA) | reinterpret_cast<uintptr_t>(c.SFB) |
                         reinterpret_cast<uintptr_t>(p.D) | reinterpret_cast<uintptr_t>(p.bias) |
-                        reinterpret_cast<uintptr_t>(p.residual);
+                        reinterpret_cast<uintptr_t>(p.residual) | reinterpret_cast<uintptr_t>(p.out4);
   if ((all & 15) || ((reinterpret_cast<uintptr_t>(p.alpha) | reinterpret_cast<uintptr_t>(p.offsets)) & 3)) {
     set_error("%s: operands, scales, bias, residual and output must be 16-byte aligned, alpha and offsets 4-byte", c.who);
     return B2_ERR_INVALID_ARGUMENT;
@@ -987,6 +1073,44 @@ extern "C" int b2_nvfp4_grouped_gemm(const void* A, const void* B, const void* S
   if (rows == 0) return B2_OK;
   if (!offsets_dev) {
     set_error("b2_nvfp4_grouped_gemm: null pointer argument");
+    return B2_ERR_INVALID_ARGUMENT;
+  }
+  c.sfa_tiles = rows / 128 + groups;
+  if (int rc = grouped_status_words(&c.p.status)) return rc;
+  return run_grouped(c, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int b2_nvfp4_grouped_gemm_gated(const void* A, const void* B, const void* SFA, const void* SFB,
+                                           const float* alpha_dev, const int32_t* offsets_dev, const float* gs_dev,
+                                           void* out, void* sf, int rows, int groups, int inner, int K, int dtype,
+                                           void* stream) {
+  using namespace b2;
+  GroupedCall c = {};
+  c.who = "b2_nvfp4_grouped_gemm_gated";
+  if (inner < 128 || inner % 128 != 0 || inner > (1 << 29)) {
+    set_error("b2_nvfp4_grouped_gemm_gated: inner=%d: need a positive multiple of 128", inner);
+    return B2_ERR_INVALID_ARGUMENT;
+  }
+  c.A = A;
+  c.B = B;
+  c.SFA = SFA;
+  c.SFB = SFB;
+  c.K = K;
+  c.p.alpha = alpha_dev;
+  c.p.offsets = offsets_dev;
+  c.p.gs = gs_dev;
+  c.p.out4 = static_cast<uint8_t*>(out);
+  c.p.sf_out = static_cast<uint8_t*>(sf);
+  c.p.rows = rows;
+  c.p.groups = groups;
+  c.p.N = 2 * inner;
+  c.p.act = B2_ACT_NONE;
+  c.p.fp16 = dtype == B2_DTYPE_F16;
+  c.p.wait_budget_ns = kWaitBudgetNs;
+  if (int rc = check_product(c, dtype)) return rc;
+  if (rows == 0) return B2_OK;
+  if (!offsets_dev || !gs_dev || !out || !sf || (reinterpret_cast<uintptr_t>(gs_dev) & 3) || (reinterpret_cast<uintptr_t>(sf) & 15)) {
+    set_error("b2_nvfp4_grouped_gemm_gated: null or misaligned pointer argument");
     return B2_ERR_INVALID_ARGUMENT;
   }
   c.sfa_tiles = rows / 128 + groups;

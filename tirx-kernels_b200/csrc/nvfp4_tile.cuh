@@ -272,14 +272,15 @@ __host__ __device__ constexpr uint32_t instr_desc(int m, int n) {
 // AM: rows of A the TMA writes per stage.  The MMA always reads 128 rows; with AM < 128 (M <= AM) the
 // rows past AM are whatever follows in the stage, which only reaches accumulator rows nobody reads,
 // and the shared memory saved buys more stages in flight.
-template <int CG, int BN, int STAGES, int TMA_OUT = 0, int AM = kBlockM>
+// SFB: 128-row scale chunks of B a stage holds when they are more than BN's (0: BN's).
+template <int CG, int BN, int STAGES, int TMA_OUT = 0, int AM = kBlockM, int SFB = 0>
 struct SmemLayout {
   static constexpr int kBRows = BN / CG;                       // rows of B held by one CTA
   static constexpr int kChunks = BN / 128 > 0 ? BN / 128 : 1;  // 128-row scale chunks of B
   static constexpr int kABytes = AM * 128;
   static constexpr int kBBytes = kBRows * 128;
   static constexpr int kSfaBytes = 4 * 512;                    // 4 K-blocks of 64, 512 B each
-  static constexpr int kSfbBytes = kChunks * 4 * 512;
+  static constexpr int kSfbBytes = (SFB ? SFB : kChunks) * 4 * 512;
   static constexpr int kStageBytes = kABytes + kBBytes + kSfaBytes + kSfbBytes;
   static constexpr int kSfCols = 16 + 16 * kChunks;            // TMEM columns of one stage's scales
   static constexpr int kBarrierBytes = 512;

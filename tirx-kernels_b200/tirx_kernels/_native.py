@@ -15,6 +15,7 @@ SF_LAYOUT_CODES = {"linear": 0, "128x4": 1, "8x4": 2}
 SCALE_FORMAT_CODES = {"e4m3": 0, "ue8m0": 1}
 ACTIVATION_CODES = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 MAX_GROUPS = 384  # groups (experts) of one grouped launch
+MAX_TOPK = 32     # experts of one token
 MUFU_OPS = {"rcp_ftz": 0, "rsqrt_ftz": 1, "lg2": 2, "ex2": 3, "ex2_ftz": 4,
             # the quantizer's SiLU as its kernel computes it / with div.rn.f32 throughout
             "silu": 5, "silu_div_rn": 6}
@@ -43,11 +44,13 @@ MAIN_SIGNATURES = {
     "b2_nvfp4_gemm_small_m_noalloc_status": (_i, [_vp]),
     "b2_nvfp4_gemm_epilogue": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
     "b2_nvfp4_grouped_gemm": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp]),
+    "b2_nvfp4_grouped_gemm_gated": (_i, [_vp] * 9 + [_i] * 5 + [_vp]),
     "b2_nvfp4_grouped_gemm_set_variant": (_i, [_i]),
     "b2_nvfp4_grouped_gemm_status": (_i, [_vp]),
     "b2_nvfp4_quantize_grouped": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp]),
     "b2_nvfp4_grouped_sf_bytes": (_i64, [_i, _i, _i]),
     "b2_moe_plan": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _vp]),
+    "b2_moe_dispatch": (_i, [_vp] * 8 + [_i] * 5 + [_vp]),
     "b2_moe_combine": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
     "b2_moe_expert_ffn": (_i, [_vp] * 14 + [_i64] + [_i] * 6 + [_vp]),
     "b2_moe_expert_ffn_workspace_bytes": (_i64, [_i, _i, _i, _i, _i]),

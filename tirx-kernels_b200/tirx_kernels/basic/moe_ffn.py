@@ -4,9 +4,9 @@
 NVFP4 block quantizer with a fixed encode scale per expert, the products are ``nvfp4_grouped_gemm``, intermediates are in
 the 16-bit type of ``x``.  Experts outside ``[0, experts)`` are dropped; a token may name an expert twice.
 
-``expert_ffn`` is the whole of it (six launches, one C call, no host synchronisation: it can be captured into a CUDA
-graph after a first call); ``plan`` and ``combine`` are its first and last step on their own, with
-``nvfp4_quantize_grouped`` and ``nvfp4_grouped_gemm`` between them.
+``expert_ffn`` is the whole of it (one C call of four to six launches, no host synchronisation: it can be captured into a
+CUDA graph after a first call); ``plan``, ``dispatch``, ``gated_product`` and ``combine`` are its steps on their own, next to
+``nvfp4_quantize_grouped`` and ``nvfp4_grouped_gemm``.
 """
 
 from __future__ import annotations
@@ -98,6 +98,57 @@ def plan(ids, experts: int):
     position = torch.empty_like(ids)
     _native.call("b2_moe_plan", device, ids, offsets, row_token, position, tokens, topk, experts)
     return offsets, row_token, position
+
+
+def dispatch(x, ids, gs):
+    """``plan`` and the quantizer in one: every row of x [tokens, hidden] in NVFP4 for each of its experts.
+
+    ``gs`` fp32 [experts], the encode scales.  Returns (packed [tokens * topk, hidden/2], scale tiles, offsets, position)."""
+    import torch
+
+    if x.ndim != 2 or ids.ndim != 2 or not 1 <= ids.shape[1] <= _native.MAX_TOPK:
+        raise ValueError(f"x must be [tokens, hidden], ids [tokens, topk] with 1 <= topk <= {_native.MAX_TOPK}")
+    (tokens, hidden), topk, experts = x.shape, ids.shape[1], gs.numel()
+    dtype = _operator.dtype_name(x.dtype)
+    if hidden < 64 or hidden % 64 or not 1 <= experts <= _native.MAX_GROUPS:
+        raise ValueError(f"hidden={hidden} must be a multiple of 64, experts={experts} in 1..{_native.MAX_GROUPS}")
+    spec = _checks.tensor_spec
+    device = _checks.require_tensors((spec("x", dtype, (tokens, hidden)), spec("ids", "int32", (tokens, topk)),
+                                      spec("gs", "float32", (experts,))), (x, ids, gs))
+    rows = tokens * topk
+    out = torch.empty(rows, hidden // 2, dtype=torch.uint8, device=x.device)
+    sf = torch.empty(_checks.grouped_sf_numel(rows, experts, hidden), dtype=torch.uint8, device=x.device)
+    offsets = torch.zeros(experts + 1, dtype=torch.int32, device=x.device)
+    position, row_token = torch.empty_like(ids), torch.empty(rows, dtype=torch.int32, device=x.device)
+    _native.call("b2_moe_dispatch", device, x, ids, gs, offsets, row_token, position, out, sf, tokens, topk, experts, hidden,
+                 _native.DTYPE_CODES[dtype])
+    return out, sf, offsets, position
+
+
+def gated_product(A, SFA, offsets, w1, sf1, alpha, gs, dtype: str = "bfloat16"):
+    """SiLU(gate) * up of ``[gate | up] = alpha[g] * A . w1[g]^T``, quantized with ``gs[g]``: (packed [rows, inner/2], scale tiles).
+
+    The bytes are those of ``nvfp4_grouped_gemm`` to `dtype` followed by ``nvfp4_quantize_grouped`` with ``fuse_silu``;
+    ``w1`` [groups, 2 * inner, hidden/2], inner a multiple of 128.  Rows that no group has are left undefined."""
+    import torch
+
+    if A.ndim != 2 or w1.ndim != 3 or w1.shape[1] % 256 or not w1.shape[1]:
+        raise ValueError("A must be [rows, hidden / 2], w1 [groups, 2 * inner, hidden / 2] with inner a multiple of 128")
+    (rows, half), (groups, gate_up, _) = A.shape, w1.shape
+    inner, hidden = gate_up // 2, half * 2
+    if hidden < 64 or hidden % 64 or not 1 <= groups <= _native.MAX_GROUPS or dtype not in _operator.DTYPES:
+        raise ValueError(f"hidden={hidden}, groups={groups}, dtype={dtype} outside the domain")
+    spec = _checks.tensor_spec
+    device = _checks.require_tensors(
+        (spec("A", "uint8", (rows, half)), spec("SFA", "uint8", _checks.grouped_sf_numel(rows, groups, hidden)),
+         spec("offsets", "int32", (groups + 1,)), spec("w1", "uint8", (groups, gate_up, half)),
+         spec("sf1", "uint8", groups * _checks.sf_numel(gate_up, hidden // 16, "128x4")), spec("alpha", "float32", (groups,)),
+         spec("gs", "float32", (groups,))), (A, SFA, offsets, w1, sf1, alpha, gs))
+    out = torch.empty(rows, inner // 2, dtype=torch.uint8, device=A.device)
+    sf = torch.empty(_checks.grouped_sf_numel(rows, groups, inner), dtype=torch.uint8, device=A.device)
+    _native.call("b2_nvfp4_grouped_gemm_gated", device, A, w1, SFA, sf1, alpha, offsets, gs, out, sf, rows, groups, inner,
+                 hidden, _native.DTYPE_CODES[dtype])
+    return out, sf
 
 
 def combine(y, position, gates, residual=None, out=None):
