@@ -356,11 +356,14 @@ __global__ void __launch_bounds__(kDispatchThreads) moe_dispatch_kernel(const __
       }
     }
     if (blockIdx.x == 0) {
-      for (int e = t; e <= p.experts; e += blockDim.x) {
-        int below = 0;
-        for (int j = 0; j < n; ++j) below += all_ids[j] < e;
-        p.offsets[e] = below;
-      }
+      __shared__ int start[kMaxGroups + 1];
+      for (int e = t; e <= p.experts; e += blockDim.x) start[e] = 0;
+      __syncthreads();
+      for (int j = t; j < n; j += blockDim.x) atomicAdd(start + all_ids[j], 1);  // integers: no order to matter
+      __syncthreads();
+      if (warp == 0) scan_experts(start, p.experts, lane);
+      __syncthreads();
+      for (int e = t; e <= p.experts; e += blockDim.x) p.offsets[e] = start[e];
     }
     __syncthreads();
   }
