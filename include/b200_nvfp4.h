@@ -384,6 +384,9 @@ int b2_gated_add_rmsnorm_fp4quant(const void* x, const void* residual, const voi
                                   int H, int rows_per_gate, float residual_scale, float eps, int in_dtype, int quantize,
                                   int swizzled, void* stream);
 
+/* Reads and clears the status word of its bounded waits on the current device, as b2_nvfp4_gemm_status. */
+int b2_gated_add_rmsnorm_fp4quant_status(void* stream);
+
 /*
  * In-kernel role timers of b2_nvfp4_gemm (observability; the reference's nearest analogue is the
  * u64 event buffer of tirx_kernels/basic/allgather_gemm.py:48-53).  `enable` != 0 makes later

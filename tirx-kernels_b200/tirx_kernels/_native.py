@@ -54,6 +54,7 @@ MAIN_SIGNATURES = {
     "b2_moe_combine": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
     "b2_moe_expert_ffn": (_i, [_vp] * 14 + [_i64] + [_i] * 6 + [_vp]),
     "b2_moe_expert_ffn_workspace_bytes": (_i64, [_i, _i, _i, _i, _i]),
+    "b2_gated_add_rmsnorm_fp4quant_status": (_i, [_vp]),
     "b2_gated_add_rmsnorm_fp4quant": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _f, _f, _i, _i, _i, _vp]),
     "b2_nvfp4_gemm_set_wait_budget_ms": (_i, [_i]),
     "b2_nvfp4_gemm_inject_test_fault": (_i, [_i]),
@@ -250,6 +251,10 @@ def nvfp4_grouped_gemm_set_variant(variant: int) -> None:
 
 def nvfp4_grouped_gemm_status() -> None:
     check(lib().b2_nvfp4_grouped_gemm_status(current_stream_ptr()), "b2_nvfp4_grouped_gemm_status")
+
+
+def gated_add_rmsnorm_fp4quant_status() -> None:
+    check(lib().b2_gated_add_rmsnorm_fp4quant_status(current_stream_ptr()), "b2_gated_add_rmsnorm_fp4quant_status")
 
 
 def peer_alloc(nbytes: int) -> int:

@@ -99,6 +99,8 @@ def run_test(input_dtype: str, M: int, H: int, quantize: bool = True, swizzled: 
         y = torch.full_like(x, float("nan"))
         ex(x, residual, w_post, g, w_pre, out, y, None, None, residual_scale, eps)
     want_h, want_y = expected(x, residual, w_post, g, w_pre, rows_per_gate, residual_scale, eps, h=out)
+    torch.cuda.synchronize()
+    _native.gated_add_rmsnorm_fp4quant_status()
     # h: one rounding, and fp32 arithmetic on terms up to |residual| + |u|
     step = torch.finfo(x.dtype).eps
     terms = want_h.abs() + 2 * residual.double().abs()
@@ -164,6 +166,10 @@ def _cfg(input_dtype, M, H, quantize=True, swizzled=True, rows_per_gate=1, post=
 
 
 CONFIGS = [
+    _cfg("bfloat16", 3000, 528, rows_per_gate=7),
+    _cfg("float16", 3001, 7168, quantize=False, rows_per_gate=1000),
+    _cfg("bfloat16", 1200, 16384, swizzled=False, gate=False),
+    _cfg("float16", 5000, 1040, post=False, gate=False),
     _cfg("bfloat16", 1, 8192),
     _cfg("bfloat16", 3, 16, gate=False),
     _cfg("float16", 500, 5136, swizzled=False, gate=False),
@@ -173,6 +179,10 @@ CONFIGS = [
     _cfg("float16", 257, 7168, quantize=False, gate=False, post=False),
 ]
 BENCH_CONFIGS = [
+    _cfg("bfloat16", 3000, 528, rows_per_gate=7),
+    _cfg("float16", 3001, 7168, quantize=False, rows_per_gate=1000),
+    _cfg("bfloat16", 1200, 16384, swizzled=False, gate=False),
+    _cfg("float16", 5000, 1040, post=False, gate=False),
     _cfg("bfloat16", 1, 8192),
     _cfg("bfloat16", 8192, 7168, rows_per_gate=2048),
     _cfg("bfloat16", 8192, 7168, quantize=False, rows_per_gate=2048),
