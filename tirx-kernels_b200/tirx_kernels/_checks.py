@@ -112,21 +112,31 @@ def tensor_spec(name: str, dtype: str, shape, optional: bool = False) -> tuple:
     return name, getattr(torch, dtype), shape, optional
 
 
+_torch = None
+
+
 def require_tensors(specs, tensors) -> int:
     """ValueError unless every tensor is what its spec says, contiguous and on the current device; returns that device.
 
     On the launch path of calls that take ten microseconds on the GPU: one pass over plain attributes, and the search for
     what is wrong only when something is."""
-    import torch
+    global _torch
+    if _torch is None:
+        import torch
 
-    device = torch.cuda.current_device() if torch.cuda.is_initialized() else -1
+        _torch = torch
+    device = _torch._C._cuda_getDevice() if _torch.cuda.is_initialized() else -2  # no device yet: no tensor is there
     for spec, t in zip(specs, tensors):
-        if t is None and spec[3]:
+        _, dtype, shape, optional = spec
+        if t is None and optional:
             continue
-        shape = spec[2]
-        if (not isinstance(t, torch.Tensor) or t.dtype is not spec[1] or t.get_device() != device or not t.is_contiguous()
-                or (t.shape != shape if shape.__class__ is tuple else t.numel() != shape) or device < 0):
-            _refuse(spec, t, device)
+        try:
+            if (t.dtype is dtype and t.get_device() == device and t.is_contiguous()
+                    and (t.shape == shape if shape.__class__ is tuple else t.numel() == shape)):
+                continue
+        except AttributeError:
+            pass
+        _refuse(spec, t, device)
     return device
 
 

@@ -234,12 +234,12 @@ def nvfp4_gemm_small_m_noalloc(A, B, SFA, SFB, alpha, D, M: int, N: int, K: int)
 
 
 # ---- the feed-forward operators: checked argument by argument in their modules (_checks.require_tensors) ----
-def call(symbol: str, device: int, *args) -> None:
-    """`symbol` with tensors as their addresses (None as null), on the current stream of `device`, the current device."""
+def call(symbol: str, device: int, tensors, *sizes) -> None:
+    """`symbol` of `tensors` as their addresses (None as null) and `sizes`, on the current stream of `device`, the current device."""
     import torch
 
-    status = getattr(_MAIN or lib(), symbol)(
-        *[a.data_ptr() if isinstance(a, torch.Tensor) else a for a in args], torch._C._cuda_getCurrentRawStream(device))
+    status = getattr(_MAIN or lib(), symbol)(*[None if t is None else t.data_ptr() for t in tensors], *sizes,
+                                             torch._C._cuda_getCurrentRawStream(device))
     if status != OK:
         check(status, symbol)
 

@@ -46,9 +46,9 @@ class _Executable:
     def __call__(self, x, residual, w_post, gate, w_pre, residual_out, y, sf, global_scale, residual_scale: float, eps: float) -> None:
         if not self.quantize and (sf is not None or global_scale is not None):
             raise ValueError("sf and global_scale belong to the quantized form")
-        device = _checks.require_tensors(self.specs, (x, residual, w_post, gate, w_pre, residual_out, y, sf, global_scale))
-        _native.call("b2_gated_add_rmsnorm_fp4quant", device, x, residual, w_post, gate, w_pre, residual_out, y, sf, global_scale,
-                     *self.sizes, residual_scale, eps, *self.codes)
+        tensors = x, residual, w_post, gate, w_pre, residual_out, y, sf, global_scale
+        _native.call("b2_gated_add_rmsnorm_fp4quant", _checks.require_tensors(self.specs, tensors), tensors, *self.sizes,
+                     residual_scale, eps, *self.codes)
 
 
 def get_kernel(input_dtype: str, M: int, H: int, quantize: bool = True, swizzled: bool = True, rows_per_gate: int = 1, **kwargs) -> KernelHandle:

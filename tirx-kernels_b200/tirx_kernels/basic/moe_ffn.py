@@ -96,7 +96,7 @@ def plan(ids, experts: int):
     offsets = torch.empty(experts + 1, dtype=torch.int32, device=ids.device)
     row_token = torch.empty(tokens * topk, dtype=torch.int32, device=ids.device)
     position = torch.empty_like(ids)
-    _native.call("b2_moe_plan", device, ids, offsets, row_token, position, tokens, topk, experts)
+    _native.call("b2_moe_plan", device, (ids, offsets, row_token, position), tokens, topk, experts)
     return offsets, row_token, position
 
 
@@ -120,7 +120,7 @@ def dispatch(x, ids, gs):
     sf = torch.empty(_checks.grouped_sf_numel(rows, experts, hidden), dtype=torch.uint8, device=x.device)
     offsets = torch.zeros(experts + 1, dtype=torch.int32, device=x.device)
     position, row_token = torch.empty_like(ids), torch.empty(rows, dtype=torch.int32, device=x.device)
-    _native.call("b2_moe_dispatch", device, x, ids, gs, offsets, row_token, position, out, sf, tokens, topk, experts, hidden,
+    _native.call("b2_moe_dispatch", device, (x, ids, gs, offsets, row_token, position, out, sf), tokens, topk, experts, hidden,
                  _native.DTYPE_CODES[dtype])
     return out, sf, offsets, position
 
@@ -146,7 +146,7 @@ def gated_product(A, SFA, offsets, w1, sf1, alpha, gs, dtype: str = "bfloat16"):
          spec("gs", "float32", (groups,))), (A, SFA, offsets, w1, sf1, alpha, gs))
     out = torch.empty(rows, inner // 2, dtype=torch.uint8, device=A.device)
     sf = torch.empty(_checks.grouped_sf_numel(rows, groups, inner), dtype=torch.uint8, device=A.device)
-    _native.call("b2_nvfp4_grouped_gemm_gated", device, A, w1, SFA, sf1, alpha, offsets, gs, out, sf, rows, groups, inner,
+    _native.call("b2_nvfp4_grouped_gemm_gated", device, (A, w1, SFA, sf1, alpha, offsets, gs, out, sf), rows, groups, inner,
                  hidden, _native.DTYPE_CODES[dtype])
     return out, sf
 
@@ -167,7 +167,7 @@ def combine(y, position, gates, residual=None, out=None):
     device = _checks.require_tensors(
         (spec("y", dtype, (rows, n)), spec("position", "int32", (tokens, topk)), spec("gates", "float32", (tokens, topk)),
          spec("residual", dtype, (tokens, n), True), spec("out", dtype, (tokens, n))), (y, position, gates, residual, out))
-    _native.call("b2_moe_combine", device, y, position, gates, residual, out, rows, tokens, topk, n, _native.DTYPE_CODES[dtype])
+    _native.call("b2_moe_combine", device, (y, position, gates, residual, out), rows, tokens, topk, n, _native.DTYPE_CODES[dtype])
     return out
 
 
@@ -202,9 +202,9 @@ def expert_ffn(x, ids, gates, weights: ExpertWeights, *, residual=None, out=None
                          f"{workspace.numel()} of {workspace.dtype} on {workspace.device}")
     if weights.w1.get_device() != device:
         raise ValueError(f"weights are on {weights.w1.device}, but the current device is cuda:{device}")
-    _native.call("b2_moe_expert_ffn", device, x, ids, gates, weights.w1, weights.sf1, weights.alpha1, weights.gs1, weights.w2,
-                 weights.sf2, weights.alpha2, weights.gs2, residual, out, workspace, workspace.numel(), *sizes,
-                 _native.DTYPE_CODES[dtype])
+    _native.call("b2_moe_expert_ffn", device,
+                 (x, ids, gates, weights.w1, weights.sf1, weights.alpha1, weights.gs1, weights.w2, weights.sf2, weights.alpha2,
+                  weights.gs2, residual, out, workspace), workspace.numel(), *sizes, _native.DTYPE_CODES[dtype])
     return out
 
 

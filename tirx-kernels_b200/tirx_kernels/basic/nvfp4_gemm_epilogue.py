@@ -43,8 +43,8 @@ class _Runner:
         self.sizes = M, N, K, _native.DTYPE_CODES[out_dtype], _native.ACTIVATION_CODES[activation]
 
     def __call__(self, A, B, SFA, SFB, alpha, bias, residual, D) -> None:
-        device = _checks.require_tensors(self.specs, (A, B, SFA, SFB, alpha, bias, residual, D))
-        _native.call("b2_nvfp4_gemm_epilogue", device, A, B, SFA, SFB, alpha, bias, residual, D, *self.sizes)
+        tensors = A, B, SFA, SFB, alpha, bias, residual, D
+        _native.call("b2_nvfp4_gemm_epilogue", _checks.require_tensors(self.specs, tensors), tensors, *self.sizes)
 
 
 def get_kernel(M: int, N: int, K: int, activation: str = "none", out_dtype: str = "bfloat16", **kwargs) -> KernelHandle:

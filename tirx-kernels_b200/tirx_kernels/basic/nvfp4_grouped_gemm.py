@@ -40,8 +40,8 @@ class _Runner:
         self.sizes = rows, groups, N, K, _native.DTYPE_CODES[out_dtype], _native.ACTIVATION_CODES[activation]
 
     def __call__(self, A, B, SFA, SFB, alpha, offsets, bias, D) -> None:
-        device = _checks.require_tensors(self.specs, (A, B, SFA, SFB, alpha, offsets, bias, D))
-        _native.call("b2_nvfp4_grouped_gemm", device, A, B, SFA, SFB, alpha, offsets, bias, D, *self.sizes)
+        tensors = A, B, SFA, SFB, alpha, offsets, bias, D
+        _native.call("b2_nvfp4_grouped_gemm", _checks.require_tensors(self.specs, tensors), tensors, *self.sizes)
 
 
 def get_kernel(rows: int, groups: int, N: int, K: int, activation: str = "none", out_dtype: str = "bfloat16", **kwargs) -> KernelHandle:

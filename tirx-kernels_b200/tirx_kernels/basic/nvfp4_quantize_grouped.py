@@ -38,8 +38,8 @@ class _Executable:
         self.sizes = in_rows, rows, groups, k, _native.DTYPE_CODES[dtype], int(fuse_silu)
 
     def __call__(self, x, index, offsets, out, sf, global_scale) -> None:
-        device = _checks.require_tensors(self.specs, (x, index, offsets, out, sf, global_scale))
-        _native.call("b2_nvfp4_quantize_grouped", device, x, index, offsets, out, sf, global_scale, *self.sizes)
+        tensors = x, index, offsets, out, sf, global_scale
+        _native.call("b2_nvfp4_quantize_grouped", _checks.require_tensors(self.specs, tensors), tensors, *self.sizes)
 
 
 def get_kernel(dtype: str, in_rows: int, rows: int, groups: int, k: int, fuse_silu: bool = False, **kwargs) -> KernelHandle:
