@@ -968,6 +968,10 @@ int run_gated(int variant, const GroupedCall& c, cudaStream_t s) {
 }
 
 int run_grouped(const GroupedCall& c, cudaStream_t s) {
+  if (!encode_tiled_fn()) {
+    set_error("%s: cuTensorMapEncodeTiled is not available from this driver", c.who);
+    return B2_ERR_CUDA;
+  }
   const int sms = device_sm_count();
   if (sms <= 0) return B2_ERR_CUDA;
   int variant = g_grouped_variant.load(std::memory_order_relaxed);
@@ -1009,10 +1013,6 @@ int check_product(const GroupedCall& c, int out_dtype) {
   if ((all & 15) || ((reinterpret_cast<uintptr_t>(p.alpha) | reinterpret_cast<uintptr_t>(p.offsets)) & 3)) {
     set_error("%s: operands, scales, bias, residual and output must be 16-byte aligned, alpha and offsets 4-byte", c.who);
     return B2_ERR_INVALID_ARGUMENT;
-  }
-  if (!encode_tiled_fn()) {
-    set_error("%s: cuTensorMapEncodeTiled is not available from this driver", c.who);
-    return B2_ERR_CUDA;
   }
   return B2_OK;
 }

@@ -210,8 +210,8 @@ def expert_ffn(x, ids, gates, weights: ExpertWeights, *, residual=None, out=None
 
 class _Executable:
     def __init__(self, tokens: int, topk: int, experts: int, hidden: int, inner: int, dtype: str):
-        if tokens < 0 or topk < 1:
-            raise ValueError(f"tokens must be >= 0 and topk >= 1, got {tokens}, {topk}")
+        if tokens < 0 or not 1 <= topk <= _native.MAX_TOPK:
+            raise ValueError(f"tokens must be >= 0 and topk in 1..{_native.MAX_TOPK}, got {tokens}, {topk}")
         if not 1 <= experts <= _native.MAX_GROUPS or hidden < 64 or hidden % 64 or inner < 64 or inner % 64:
             raise ValueError(f"experts={experts} hidden={hidden} inner={inner}: need 1..{_native.MAX_GROUPS} experts, multiples of 64")
         if dtype not in _operator.DTYPES:

@@ -85,22 +85,23 @@ def prepare_data(rows: int, groups: int, N: int, K: int, out_dtype: str = "bfloa
 
 
 def expected(A, B, SFA, SFB, alpha, offsets, bias, activation: str):
-    """The formula in float64, group by group; NaN in rows that no group has."""
+    """(the formula in float64 group by group, NaN in rows that no group has; the magnitude of its terms)."""
     import torch
 
     groups, N, half = B.shape
     want = torch.full((A.shape[0], N), float("nan"), dtype=torch.float64, device=A.device)
+    size = torch.zeros_like(want)
     per = SFB.numel() // groups
     ends = offsets.tolist()
     for g, (first, last) in enumerate(zip(ends, ends[1:])):
         rows = torch.arange(last - first, device=A.device)
         a = _checks.dequantize_rows(A[first:last], SFA, (first // 128 + g) * 128 + rows)
         b = _checks.dequantize_rows(B[g], SFB[g * per:(g + 1) * per], torch.arange(N, device=A.device))
-        d = a @ b.T * alpha[g].double()
+        d, terms = a @ b.T * alpha[g].double(), a.abs() @ b.abs().T * alpha[g].double().abs()
         if bias is not None:
-            d = d + bias[g].double()
-        want[first:last] = _checks.activation(d, activation)
-    return want
+            d, terms = d + bias[g].double(), terms + bias[g].double().abs()
+        want[first:last], size[first:last] = _checks.activation(d, activation), terms
+    return want, size
 
 
 def run_test(rows: int, groups: int, N: int, K: int, activation: str = "none", out_dtype: str = "bfloat16", bias: bool = True,
@@ -115,13 +116,13 @@ def run_test(rows: int, groups: int, N: int, K: int, activation: str = "none", o
     compile_kernel(get_kernel(rows=rows, groups=groups, N=N, K=K, activation=activation, out_dtype=out_dtype))(*data, D)
     torch.cuda.synchronize()
     _native.nvfp4_grouped_gemm_status()
-    want = expected(*data, activation)
+    want, size = expected(*data, activation)
     nowhere = want.isnan()
     assert torch.equal(D.isnan(), nowhere), "nvfp4_grouped_gemm wrote rows that no group has, or left out some that one has"
     if nowhere.all():
         return
-    want, got = want[~nowhere], D[~nowhere].double()
-    excess = ((got - want).abs() - tolerance(want, out_dtype)).max().item()
+    want, size, got = want[~nowhere], size[~nowhere], D[~nowhere].double()
+    excess = ((got - want).abs() - tolerance(want, size, K, out_dtype)).max().item()
     assert excess <= 0, f"nvfp4_grouped_gemm is off by {excess:.3e} more than fp32 sums and one rounding allow"
 
 
