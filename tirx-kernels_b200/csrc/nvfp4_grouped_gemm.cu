@@ -110,16 +110,22 @@ __device__ __forceinline__ float gate_sigmoid(float v, float c1, float c2) {
   return v * rcp_approx_ftz(1.0f + e);
 }
 // v Phi(v) with the upper tail of the normal distribution by Abramowitz & Stegun 7.1.26 (absolute error 1.5e-7):
-// erfc(z) = (a1 t + .. + a5 t^5) e^(-z^2), t = 1 / (1 + p z), z = |v| / sqrt 2.
-__device__ __forceinline__ float gelu_erf(float v) {
-  const float z = fabsf(v) * 0.70710678118654752f;
-  const float t = rcp_approx_ftz(fmaf(0.3275911f, z, 1.0f));
-  float poly = fmaf(1.061405429f, t, -1.453152027f);
-  poly = fmaf(poly, t, 1.421413741f);
-  poly = fmaf(poly, t, -0.284496736f);
-  poly = fmaf(poly, t, 0.254829592f);
-  const float half_tail = 0.5f * poly * t * ex2_approx_ftz(z * z * -1.4426950408889634f);
-  return v * (v >= 0.0f ? 1.0f - half_tail : half_tail);
+// erfc(z) = (a1 t + .. + a5 t^5) e^(-z^2), t = 1 / (1 + p z), z = |v| / sqrt 2.  Two values at once: packed arithmetic, and
+// one reciprocal of the product of both denominators (the MUFU is what bounds this step); z is capped where the tail
+// has long been zero, so that the product stays finite and one value's infinity or NaN does not reach the other.
+__device__ __forceinline__ float2 gelu_erf(float2 v) {
+  const float2 z = make_float2(fminf(fabsf(v.x) * 0.70710678118654752f, 64.0f), fminf(fabsf(v.y) * 0.70710678118654752f, 64.0f));
+  const float2 d = fma_f32x2(make_float2(0.3275911f, 0.3275911f), z, make_float2(1.0f, 1.0f));
+  const float both = rcp_approx_ftz(d.x * d.y);
+  const float2 t = mul_f32x2(make_float2(both, both), make_float2(d.y, d.x));
+  float2 poly = fma_f32x2(make_float2(1.061405429f, 1.061405429f), t, make_float2(-1.453152027f, -1.453152027f));
+  poly = fma_f32x2(poly, t, make_float2(1.421413741f, 1.421413741f));
+  poly = fma_f32x2(poly, t, make_float2(-0.284496736f, -0.284496736f));
+  poly = fma_f32x2(poly, t, make_float2(0.254829592f, 0.254829592f));
+  const float2 w = mul_f32x2(mul_f32x2(z, z), make_float2(-1.4426950408889634f, -1.4426950408889634f));
+  const float2 e = make_float2(ex2_approx_ftz(w.x), ex2_approx_ftz(w.y));
+  const float2 tail = mul_f32x2(mul_f32x2(poly, t), mul_f32x2(e, make_float2(0.5f, 0.5f)));
+  return make_float2(v.x * (v.x >= 0.0f ? 1.0f - tail.x : tail.x), v.y * (v.y >= 0.0f ? 1.0f - tail.y : tail.y));
 }
 
 // Not the read-only path: the residual may be the output's own memory (every word is read before it is written, by
@@ -163,7 +169,11 @@ __device__ __forceinline__ void activate(int act, uint32_t* v) {
     for (int i = 0; i < COLS; ++i) v[i] = __float_as_uint(gate_sigmoid(__uint_as_float(v[i]), c1, c2));
   } else if (act == B2_ACT_GELU) {
 #pragma unroll
-    for (int i = 0; i < COLS; ++i) v[i] = __float_as_uint(gelu_erf(__uint_as_float(v[i])));
+    for (int i = 0; i < COLS; i += 2) {
+      const float2 g = gelu_erf(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])));
+      v[i] = __float_as_uint(g.x);
+      v[i + 1] = __float_as_uint(g.y);
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < COLS; ++i) v[i] = __uint_as_float(v[i]) < 0.0f ? 0u : v[i];  // ReLU; a NaN stays one
