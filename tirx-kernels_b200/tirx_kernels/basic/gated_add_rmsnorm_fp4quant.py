@@ -179,10 +179,6 @@ CONFIGS = [
     _cfg("float16", 257, 7168, quantize=False, gate=False, post=False),
 ]
 BENCH_CONFIGS = [
-    _cfg("bfloat16", 3000, 528, rows_per_gate=7),
-    _cfg("float16", 3001, 7168, quantize=False, rows_per_gate=1000),
-    _cfg("bfloat16", 1200, 16384, swizzled=False, gate=False),
-    _cfg("float16", 5000, 1040, post=False, gate=False),
     _cfg("bfloat16", 1, 8192),
     _cfg("bfloat16", 8192, 7168, rows_per_gate=2048),
     _cfg("bfloat16", 8192, 7168, quantize=False, rows_per_gate=2048),
