@@ -202,6 +202,22 @@ __device__ __forceinline__ uint32_t pack_from_f32<BF16Tag>(float lo, float hi) {
   return r;
 }
 
+// Two values to 16 bits in one instruction.
+template <typename Tag>
+__device__ __forceinline__ uint32_t pack_pair(float2 v);
+template <>
+__device__ __forceinline__ uint32_t pack_pair<F16Tag>(float2 v) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(v.y), "f"(v.x));
+  return r;
+}
+template <>
+__device__ __forceinline__ uint32_t pack_pair<BF16Tag>(float2 v) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(v.y), "f"(v.x));
+  return r;
+}
+
 // Tree abs-max over four packed words (8 values), then the max of the two lanes as fp32.
 template <typename Tag>
 __device__ __forceinline__ uint32_t absmax_4(const uint32_t (&v)[4]) {

@@ -53,22 +53,6 @@ __device__ __forceinline__ void st_256(void* p, const uint32_t (&r)[8]) {
                : "memory");
 }
 
-// Two values to 16 bits in one instruction.
-template <typename Tag>
-__device__ __forceinline__ uint32_t pack_pair(float2 v);
-template <>
-__device__ __forceinline__ uint32_t pack_pair<F16Tag>(float2 v) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(v.y), "f"(v.x));
-  return r;
-}
-template <>
-__device__ __forceinline__ uint32_t pack_pair<BF16Tag>(float2 v) {
-  uint32_t r;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(v.y), "f"(v.x));
-  return r;
-}
-
 // Mixed-precision multiply-adds (sm_100): 16-bit factors, fp32 sum, no unpacking.
 template <typename Tag, bool HIGH>
 __device__ __forceinline__ float fma_mixed(uint32_t a, uint32_t b, float c) {

@@ -22,10 +22,10 @@
 //     multiplied (zeros, or the next group's weights) and dropped;
 //   * 32-row tiles for groups of a few rows (AM = 32) may start in any quarter of a 128-row scale tile; the scale
 //     warps move that quarter to the first place;
-//   * the epilogue takes its part of the accumulator into registers as raw fp32 and hands tensor memory back before it
-//     computes anything: bias, activation, residual and stores run beside the next tile's products.  The 256 x 256 pair
-//     has 16 epilogue warps for that (64 columns of fp32 a thread; 8 warps would need 128) and moves registers to them
-//     with setmaxnreg; with NACC == 2 the accumulator itself is double.
+//   * the epilogue runs beside the next tile's products.  Where tensor memory has room for two accumulators (NACC == 2),
+//     or a CTA has one tile, it loops over 16 columns of the held one.  The 256 x 256 pair has room for one: 16
+//     epilogue warps take it into registers as raw fp32 (64 columns a thread; 8 warps would need 128, hence setmaxnreg)
+//     and hand it back before they compute anything; the last tile, which nothing waits for, is held again.
 #include <atomic>
 
 #include "nvfp4_tile.cuh"
@@ -139,7 +139,11 @@ __device__ __forceinline__ uint4 load_residual(const uint16_t* p) {
 __device__ __forceinline__ void touch(const uint16_t* p) {
   asm volatile("{ .reg .b32 a, b, c, d; ld.global.nc.v4.b32 {a, b, c, d}, [%0]; }" ::"l"(p));
 }
-__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+// 16 columns of a row of the residual, of which `left` (a multiple of 8) are there.
+__device__ __forceinline__ void load_next(const uint16_t* p, int left, uint4 (&r)[2]) {
+  if (left > 0) r[0] = load_residual(p);
+  if (left > 8) r[1] = load_residual(p + 8);
+}
 
 // ---- the epilogue's steps, each over all of a warp's columns of one row, in place --------------------------------------
 // One step after another, with the choice of activation or type outside the loop: what a call does not use it does not
@@ -192,7 +196,7 @@ __device__ __forceinline__ void add8(uint4 r, uint32_t* v) {
 template <typename Tag, int N>
 __device__ __forceinline__ void pack(uint32_t* v) {
 #pragma unroll
-  for (int i = 0; i < N / 2; ++i) v[i] = pack_from_f32<Tag>(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+  for (int i = 0; i < N / 2; ++i) v[i] = pack_pair<Tag>(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])));
 }
 
 __device__ __forceinline__ void lds64(uint32_t addr, uint32_t* r) {
@@ -229,35 +233,23 @@ __device__ __forceinline__ void take_registers() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS));
 }
 
-// 32 gate and 32 up columns of one row -> SiLU(gate) * up in NVFP4: two blocks, with the bits that the 16-bit product
+// 16 gate and 16 up columns of one row -> a block of SiLU(gate) * up in NVFP4, with the bits that the 16-bit product
 // followed by the quantizer's fuse_silu gives (the same roundings: product to 16 bits, SiLU * up to 16 bits).
 template <typename Tag>
-__device__ __forceinline__ void gated_blocks(const GroupedParams& p, const uint32_t* v, float alpha, int group, int row,
-                                             int64_t sf_row, int col) {
-  const float gs = __ldg(p.gs + group);
-  const float rcp_gs = rcp_approx_ftz(gs), rcp6 = rcp_approx_ftz(6.0f);
-  uint32_t codes = 0;
-  uint2 packed[2];
+__device__ __forceinline__ void gated_block(const uint32_t* gate, const uint32_t* up, float alpha, float gs, uint32_t& sf_byte,
+                                            uint2& packed) {
+  uint32_t w[8];
 #pragma unroll
-  for (int b = 0; b < 2; ++b) {
-    uint32_t w[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t* g = v + 16 * b + 2 * i;
-      const uint32_t gate = pack_from_f32<Tag>(__uint_as_float(g[0]) * alpha, __uint_as_float(g[1]) * alpha);
-      const uint32_t up = pack_from_f32<Tag>(__uint_as_float(g[32]) * alpha, __uint_as_float(g[33]) * alpha);
-      w[i] = silu_and_mul_pair<Tag>(gate, up);
-    }
-    uint32_t sf_byte;
-    quantize_block<Tag>(w, gs, rcp_gs, rcp6, sf_byte, packed[b]);
-    codes |= sf_byte << (8 * b);
-  }
-  const int cols = p.N / 32;  // scale blocks of a row
-  *reinterpret_cast<uint16_t*>(p.sf_out + (col / 16 & 3) + static_cast<int64_t>(col / 64) * 512 + (sf_row & 31) * 16 +
-                               ((sf_row & 127) >> 5) * 4 + (sf_row >> 7) * (128 * static_cast<int64_t>(cols))) =
-      static_cast<uint16_t>(codes);
-  *reinterpret_cast<uint4*>(p.out4 + static_cast<int64_t>(row) * (p.N / 4) + col / 2) =
-      make_uint4(packed[0].x, packed[0].y, packed[1].x, packed[1].y);
+  for (int i = 0; i < 8; ++i)
+    w[i] = silu_and_mul_pair<Tag>(
+        pack_pair<Tag>(make_float2(__uint_as_float(gate[2 * i]) * alpha, __uint_as_float(gate[2 * i + 1]) * alpha)),
+        pack_pair<Tag>(make_float2(__uint_as_float(up[2 * i]) * alpha, __uint_as_float(up[2 * i + 1]) * alpha)));
+  quantize_block<Tag>(w, gs, rcp_approx_ftz(gs), rcp_approx_ftz(6.0f), sf_byte, packed);
+}
+// Where a row's scale of column `col` (a multiple of 16) lies, `inner` columns a row.
+__device__ __forceinline__ int64_t gated_sf_offset(int64_t sf_row, int col, int inner) {
+  return (col / 16 & 3) + static_cast<int64_t>(col / 64) * 512 + (sf_row & 31) * 16 + ((sf_row & 127) >> 5) * 4 +
+         (sf_row >> 7) * (8 * static_cast<int64_t>(inner));
 }
 
 // CG: CTAs of a tile (1 or 2).  BN: its columns.  AM: rows of A that one CTA loads and multiplies (the MMA reads 128;
@@ -402,120 +394,120 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
   // setmaxnreg stands in front of the roles of its warpgroup, inside one branch: behind a point where branches with
   // different limits meet, the compiler keeps to the lowest.
   if (warp < kGWarpScale0) {
-  if constexpr (kMoveRegisters) give_registers<kRegsIssue>();
-  if (warp == kGWarpOperands) {
-    // ================= TMA producer of the operands =================
-    if (kWarpWide || lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      bool alive = true;
-      for (int t = unit; t < num_tiles && alive; t += num_units) {
-        const Tile tile = find_tile<MODE>(p, starts, group_rows, t);
-        const int row_a = uniform(tile.first + tile.tm * kBM) + static_cast<int>(rank) * kBlockM;
-        // Gated: the first half of the tile's columns are gates, the second (the pair's second CTA's) the matching ups.
-        const int row_b = MODE == kGated ? uniform(tile.group * p.N + tile.tn * (BN / 2)) + static_cast<int>(rank) * (p.N / 2)
-                                         : uniform(tile.group * p.N + tile.tn * BN) + static_cast<int>(rank) * L::kBRows;
-        for (int ks = 0; ks < k_slabs; ++ks) {
-          if (!role_wait(empty_bar(stage), phase ^ 1u, 1u)) { alive = false; break; }
-          const uint32_t sbase = smem_base + stage * L::kStageBytes;
-          // operand bytes of both CTAs of a pair are counted on the leader's barrier
-          const uint32_t op_bar = CG == 2 ? mapa_shared(full_bar(stage), 0) : full_bar(stage);
-          if (issues()) {
-            if (leader) mbar_expect_tx(full_bar(stage), kOperandTx);
-            tma_load_2d<CG>(sbase, &map_a, ks * 128, row_a, op_bar);
-            tma_load_2d<CG>(sbase + L::kABytes, &map_b, ks * 128, row_b, op_bar);
-            if constexpr (MODE == kGated && CG == 1)
-              tma_load_2d<CG>(sbase + L::kABytes + L::kBBytes / 2, &map_b, ks * 128, row_b + p.N / 2, op_bar);
-          }
-          if constexpr (kWarpWide) __syncwarp();
-          if (++stage == STAGES) { stage = 0; phase ^= 1u; }
-        }
-      }
-    }
-  } else if (warp == kGWarpScales) {
-    // ================= TMA producer of the scale factors =================
-    if (kWarpWide || lane == 0) {
-      const int sfb_tiles = (p.N + 127) / 128;
-      int stage = 0;
-      uint32_t phase = 0;
-      bool alive = true;
-      for (int t = unit; t < num_tiles && alive; t += num_units) {
-        const Tile tile = find_tile<MODE>(p, starts, group_rows, t);
-        const int sfa_tile = uniform((tile.first >> 7) + tile.group + ((tile.tm * kBM) >> 7)) + static_cast<int>(rank);
-        const int sfb_tile = uniform(tile.group * sfb_tiles + (tile.tn * (MODE == kGated ? BN / 2 : BN)) / 128);
-        for (int ks = 0; ks < k_slabs; ++ks) {
-          if (!role_wait(empty_bar(stage), phase ^ 1u, 1u)) { alive = false; break; }
-          const uint32_t sf_smem = smem_base + stage * L::kStageBytes + L::kABytes + L::kBBytes;
-          if (issues()) {
-            mbar_expect_tx(sfload_bar(stage), kScaleTx);
-            tma_load_3d<1>(sf_smem, &map_sfa, 0, ks * 4, sfa_tile, sfload_bar(stage));
-            tma_load_3d<1>(sf_smem + L::kSfaBytes, &map_sfb, 0, ks * 4, sfb_tile, sfload_bar(stage));
-            if constexpr (MODE == kGated)
-              tma_load_3d<1>(sf_smem + L::kSfaBytes + 2048, &map_sfb, 0, ks * 4, sfb_tile + p.N / 256, sfload_bar(stage));
-          }
-          if constexpr (kWarpWide) __syncwarp();
-          if (++stage == STAGES) { stage = 0; phase ^= 1u; }
-        }
-      }
-    }
-  } else if (warp == kGWarpMma || (MMAS == 2 && warp == kGWarpMma2)) {
-    // ================= MMA issuer(s), in the leader =================
-    // Issuer `me` takes the K slabs with index % MMAS == me and adds them up in its own columns.
-    const int me = warp == kGWarpMma ? 0 : 1;
-    if (leader && (kWarpWide || lane == 0)) {
-      bool alive = true;
-      int acc = 0;
-      uint32_t acc_phase = 0;
-      int slab0 = 0;  // slabs of the tiles that are done: the ring position of this tile's first slab
-      for (int t = unit; t < num_tiles && alive; t += num_units, slab0 += k_slabs) {
-        if (!role_wait(acc_empty_bar(acc), acc_phase ^ 1u, 2u)) break;
-        tc_fence_after();
-        // A 64-wide tile uses half of a 128-row scale chunk of B: the upper half starts two columns in.
-        uint32_t sfb_half = 0;
-        if constexpr (BN == 64) sfb_half = static_cast<uint32_t>(find_tile<MODE>(p, starts, group_rows, t).tn & 1) * 2u;
-        const uint32_t acc_tmem = tmem_base + static_cast<uint32_t>((acc * MMAS + me) * BN);
-        int stage = (slab0 + me) % STAGES;
-        uint32_t phase = static_cast<uint32_t>((slab0 + me) / STAGES) & 1u;
-        bool polled = false;  // the poll issued with the previous slab found this slab's barrier complete
-        for (int ks = me; ks < k_slabs; ks += MMAS) {
-          if (!polled && !role_wait(full_bar(stage), phase, 3u)) { alive = false; break; }
-          tc_fence_after();
-          const uint32_t sbase = smem_base + stage * L::kStageBytes;
-          const uint32_t sf_tmem = tmem_base + kAccCols + stage * L::kSfCols;
-          const uint64_t a_desc = operand_desc(sbase), b_desc = operand_desc(sbase + L::kABytes);
-          int next_stage = stage + MMAS;
-          uint32_t next_phase = phase;
-          if (next_stage >= STAGES) { next_stage -= STAGES; next_phase ^= 1u; }
-          if constexpr (kWarpWide) {
-            if (elect_one()) {
-#pragma unroll
-              for (int kb = 0; kb < 4; ++kb)
-                tc_mma<CG>(acc_tmem, a_desc + 2 * kb, b_desc + 2 * kb, kIdesc, sf_tmem + kb * 4,
-                           sf_tmem + 16 + kb * 4 * L::kChunks + sfb_half, (ks >= MMAS || kb) ? 1u : 0u);
-              tc_commit_pair(empty_bar(stage));
+    if constexpr (kMoveRegisters) give_registers<kRegsIssue>();
+    if (warp == kGWarpOperands) {
+      // ================= TMA producer of the operands =================
+      if (kWarpWide || lane == 0) {
+        int stage = 0;
+        uint32_t phase = 0;
+        bool alive = true;
+        for (int t = unit; t < num_tiles && alive; t += num_units) {
+          const Tile tile = find_tile<MODE>(p, starts, group_rows, t);
+          const int row_a = uniform(tile.first + tile.tm * kBM) + static_cast<int>(rank) * kBlockM;
+          // Gated: the first half of the tile's columns are gates, the second (the pair's second CTA's) the matching ups.
+          const int row_b = MODE == kGated ? uniform(tile.group * p.N + tile.tn * (BN / 2)) + static_cast<int>(rank) * (p.N / 2)
+                                           : uniform(tile.group * p.N + tile.tn * BN) + static_cast<int>(rank) * L::kBRows;
+          for (int ks = 0; ks < k_slabs; ++ks) {
+            if (!role_wait(empty_bar(stage), phase ^ 1u, 1u)) { alive = false; break; }
+            const uint32_t sbase = smem_base + stage * L::kStageBytes;
+            // operand bytes of both CTAs of a pair are counted on the leader's barrier
+            const uint32_t op_bar = CG == 2 ? mapa_shared(full_bar(stage), 0) : full_bar(stage);
+            if (issues()) {
+              if (leader) mbar_expect_tx(full_bar(stage), kOperandTx);
+              tma_load_2d<CG>(sbase, &map_a, ks * 128, row_a, op_bar);
+              tma_load_2d<CG>(sbase + L::kABytes, &map_b, ks * 128, row_b, op_bar);
+              if constexpr (MODE == kGated && CG == 1)
+                tma_load_2d<CG>(sbase + L::kABytes + L::kBBytes / 2, &map_b, ks * 128, row_b + p.N / 2, op_bar);
             }
-            __syncwarp();
-          } else {
-            const bool more = ks + MMAS < k_slabs;  // behind the last slab the poll asks this slab's own barrier
-            const uint32_t ok = tc_slab_and_poll_next<CG>(
-                acc_tmem, a_desc, b_desc, kIdesc, sf_tmem, sf_tmem + 16 + sfb_half, 4 * L::kChunks,
-                ks >= MMAS ? 1u : 0u, empty_bar(stage), full_bar(more ? next_stage : stage),
-                more ? next_phase : phase);
-            polled = more && ok != 0;
+            if constexpr (kWarpWide) __syncwarp();
+            if (++stage == STAGES) { stage = 0; phase ^= 1u; }
           }
-          stage = next_stage;
-          phase = next_phase;
         }
-        if (!alive) break;
-        if (issues()) {
-          if constexpr (CG == 2) tc_commit_pair(acc_full_bar(acc));
-          else tc_commit<CG>(acc_full_bar(acc));
+      }
+    } else if (warp == kGWarpScales) {
+      // ================= TMA producer of the scale factors =================
+      if (kWarpWide || lane == 0) {
+        const int sfb_tiles = (p.N + 127) / 128;
+        int stage = 0;
+        uint32_t phase = 0;
+        bool alive = true;
+        for (int t = unit; t < num_tiles && alive; t += num_units) {
+          const Tile tile = find_tile<MODE>(p, starts, group_rows, t);
+          const int sfa_tile = uniform((tile.first >> 7) + tile.group + ((tile.tm * kBM) >> 7)) + static_cast<int>(rank);
+          const int sfb_tile = uniform(tile.group * sfb_tiles + (tile.tn * (MODE == kGated ? BN / 2 : BN)) / 128);
+          for (int ks = 0; ks < k_slabs; ++ks) {
+            if (!role_wait(empty_bar(stage), phase ^ 1u, 1u)) { alive = false; break; }
+            const uint32_t sf_smem = smem_base + stage * L::kStageBytes + L::kABytes + L::kBBytes;
+            if (issues()) {
+              mbar_expect_tx(sfload_bar(stage), kScaleTx);
+              tma_load_3d<1>(sf_smem, &map_sfa, 0, ks * 4, sfa_tile, sfload_bar(stage));
+              tma_load_3d<1>(sf_smem + L::kSfaBytes, &map_sfb, 0, ks * 4, sfb_tile, sfload_bar(stage));
+              if constexpr (MODE == kGated)
+                tma_load_3d<1>(sf_smem + L::kSfaBytes + 2048, &map_sfb, 0, ks * 4, sfb_tile + p.N / 256, sfload_bar(stage));
+            }
+            if constexpr (kWarpWide) __syncwarp();
+            if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+          }
         }
-        if constexpr (kWarpWide) __syncwarp();
-        if (++acc == NACC) { acc = 0; acc_phase ^= 1u; }
+      }
+    } else if (warp == kGWarpMma || (MMAS == 2 && warp == kGWarpMma2)) {
+      // ================= MMA issuer(s), in the leader =================
+      // Issuer `me` takes the K slabs with index % MMAS == me and adds them up in its own columns.
+      const int me = warp == kGWarpMma ? 0 : 1;
+      if (leader && (kWarpWide || lane == 0)) {
+        bool alive = true;
+        int acc = 0;
+        uint32_t acc_phase = 0;
+        int slab0 = 0;  // slabs of the tiles that are done: the ring position of this tile's first slab
+        for (int t = unit; t < num_tiles && alive; t += num_units, slab0 += k_slabs) {
+          if (!role_wait(acc_empty_bar(acc), acc_phase ^ 1u, 2u)) break;
+          tc_fence_after();
+          // A 64-wide tile uses half of a 128-row scale chunk of B: the upper half starts two columns in.
+          uint32_t sfb_half = 0;
+          if constexpr (BN == 64) sfb_half = static_cast<uint32_t>(find_tile<MODE>(p, starts, group_rows, t).tn & 1) * 2u;
+          const uint32_t acc_tmem = tmem_base + static_cast<uint32_t>((acc * MMAS + me) * BN);
+          int stage = (slab0 + me) % STAGES;
+          uint32_t phase = static_cast<uint32_t>((slab0 + me) / STAGES) & 1u;
+          bool polled = false;  // the poll issued with the previous slab found this slab's barrier complete
+          for (int ks = me; ks < k_slabs; ks += MMAS) {
+            if (!polled && !role_wait(full_bar(stage), phase, 3u)) { alive = false; break; }
+            tc_fence_after();
+            const uint32_t sbase = smem_base + stage * L::kStageBytes;
+            const uint32_t sf_tmem = tmem_base + kAccCols + stage * L::kSfCols;
+            const uint64_t a_desc = operand_desc(sbase), b_desc = operand_desc(sbase + L::kABytes);
+            int next_stage = stage + MMAS;
+            uint32_t next_phase = phase;
+            if (next_stage >= STAGES) { next_stage -= STAGES; next_phase ^= 1u; }
+            if constexpr (kWarpWide) {
+              if (elect_one()) {
+#pragma unroll
+                for (int kb = 0; kb < 4; ++kb)
+                  tc_mma<CG>(acc_tmem, a_desc + 2 * kb, b_desc + 2 * kb, kIdesc, sf_tmem + kb * 4,
+                             sf_tmem + 16 + kb * 4 * L::kChunks + sfb_half, (ks >= MMAS || kb) ? 1u : 0u);
+                tc_commit_pair(empty_bar(stage));
+              }
+              __syncwarp();
+            } else {
+              const bool more = ks + MMAS < k_slabs;  // behind the last slab the poll asks this slab's own barrier
+              const uint32_t ok = tc_slab_and_poll_next<CG>(
+                  acc_tmem, a_desc, b_desc, kIdesc, sf_tmem, sf_tmem + 16 + sfb_half, 4 * L::kChunks,
+                  ks >= MMAS ? 1u : 0u, empty_bar(stage), full_bar(more ? next_stage : stage),
+                  more ? next_phase : phase);
+              polled = more && ok != 0;
+            }
+            stage = next_stage;
+            phase = next_phase;
+          }
+          if (!alive) break;
+          if (issues()) {
+            if constexpr (CG == 2) tc_commit_pair(acc_full_bar(acc));
+            else tc_commit<CG>(acc_full_bar(acc));
+          }
+          if constexpr (kWarpWide) __syncwarp();
+          if (++acc == NACC) { acc = 0; acc_phase ^= 1u; }
+        }
       }
     }
-  }
   } else if (warp < kWarpEpi0) {
     if constexpr (kMoveRegisters) give_registers<kRegsScale>();
     // ================= scale warps: shared memory -> registers -> tensor memory =================
@@ -595,6 +587,7 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
   } else {
     if constexpr (kMoveRegisters) take_registers<kRegsEpilogue>();
     // ================= epilogue: lane quarter = warp & 3, column part = (warp - first) / 4 ===========
+    constexpr bool kAlwaysHold = NACC == 2 || MMAS == 2;  // see hold_tile
     const int quarter = warp & 3;
     const int part = (warp - kWarpEpi0) >> 2;
     const uint64_t store_policy = l2_policy_evict_first();
@@ -609,64 +602,34 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
     uint32_t res_phase = 0;
     int acc = 0;
     uint32_t acc_phase = 0;
-    for (int t = unit; t < num_tiles; t += num_units) {
-      const Tile tile = find_tile<MODE>(p, starts, group_rows, t);
-      const float alpha = __ldg(p.alpha + tile.group);
-      const int in_tile = static_cast<int>(rank) * kBlockM + quarter * 32;  // first row of this warp in the tile
-      const int row0 = tile.first + tile.tm * kBM + in_tile;
-      const int row = row0 + lane;
-      const int col0 = tile.tn * BN + part * kCols;
-      const bool any = in_tile < kBM && row0 < tile.last && (MODE == kGated || col0 < p.N);  // the same in the whole warp
-      const bool mine = any && row < tile.last;
-      const int64_t at = static_cast<int64_t>(row) * p.N + col0;
-      const uint16_t* bias = p.bias ? p.bias + static_cast<int64_t>(tile.group) * p.N + col0 : nullptr;
-      const uint16_t* residual = p.residual && mine ? p.residual + at : nullptr;
-      if constexpr (TMA_OUT > 0) {
-        // The residual comes by the TMA into the staging buffers, half of the rows at a time (both halves at once
-        // where there are two buffers); row-strided loads of it took 8192 x 8192 x 8192 from 199 to 277 us.
-        if (any && p.residual && lane == 0) {
-          bulk_wait_read<0>();  // the stores of the last tile have read the buffers
-          mbar_expect_tx(res_bar, 2048u * kBufs);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (h < kBufs) tma_load_2d<1>(staging + h * 2048u, &map_r, col0, row0 + 16 * h, res_bar);
-            else tma_prefetch_2d(&map_r, col0, row0 + 16 * h);
-          }
-        }
-      } else if (residual && kCols == 64) {
-        prefetch_l2(residual);
-      }
-      uint4 early[4];  // 32 columns leave room for the residual while the products run
-      if constexpr (kCols == 32) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          if (residual && col0 + 8 * c < p.N) early[c] = load_residual(residual + 8 * c);
-      }
-      if (bias && any && lane < kCols / 8 && col0 + 8 * lane < p.N) touch(bias + 8 * lane);  // into L1
-      if (!warp_wait(acc_full_bar(acc), acc_phase, 4u)) break;
-      tc_fence_after();
-      uint32_t v[kCols];
-      if (any) {
-        const uint32_t acc_tmem = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
-                                  static_cast<uint32_t>(acc * MMAS * BN + part * kCols);
-#pragma unroll
-        for (int c0 = 0; c0 < kCols; c0 += 32)
-          tmem_ld_32x32(MODE == kGated ? acc_tmem - part * 32 + c0 / 32 * (BN / 2) : acc_tmem + c0,
-                        *reinterpret_cast<uint32_t(*)[32]>(v + c0));
-        if (MMAS == 1 || !two) tmem_ld_wait();
-        if constexpr (MMAS == 2) {
-          if (two) {
-#pragma unroll
-            for (int c0 = 0; c0 < kCols; c0 += 16) {
-              uint32_t w[16];
-              tmem_ld_32x16(acc_tmem + BN + c0, w);
-              tmem_ld_wait();
-#pragma unroll
-              for (int i = 0; i < 16; ++i) v[c0 + i] = __float_as_uint(__uint_as_float(v[c0 + i]) + __uint_as_float(w[i]));
-            }
-          }
-        }
-      }
+
+    // This warp's part of a tile.
+    struct Part {
+      Tile tile;
+      float alpha;
+      int row0, row, col0;
+      bool any, mine;         // the warp has rows and columns here; the lane has a row
+      int64_t at;             // of the lane's first element in D
+      const uint16_t* bias;   // of the warp's first column, or null
+    };
+    auto part_of = [&](int t) {
+      Part w;
+      w.tile = find_tile<MODE>(p, starts, group_rows, t);
+      w.alpha = __ldg(p.alpha + w.tile.group);
+      const int in_tile = static_cast<int>(rank) * kBlockM + quarter * 32;
+      w.row0 = w.tile.first + w.tile.tm * kBM + in_tile;
+      w.row = w.row0 + lane;
+      w.col0 = w.tile.tn * BN + part * kCols;
+      w.any = in_tile < kBM && w.row0 < w.tile.last && (MODE == kGated || w.col0 < p.N);
+      w.mine = w.any && w.row < w.tile.last;
+      w.at = static_cast<int64_t>(w.row) * p.N + w.col0;
+      w.bias = p.bias ? p.bias + static_cast<int64_t>(w.tile.group) * p.N + w.col0 : nullptr;
+      if (w.bias && w.any && lane < kCols / 8 && w.col0 + 8 * lane < p.N) touch(w.bias + 8 * lane);  // into L1
+      return w;
+    };
+    // The TMA clips rows behind the last row and columns behind N, but knows nothing of groups.
+    auto whole = [&](const Part& w) { return TMA_OUT > 0 && (w.row0 + 32 <= w.tile.last || w.tile.last == p.rows); };
+    auto give_back = [&] {  // the accumulator
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
@@ -674,108 +637,271 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
         else mbar_arrive_cluster_relaxed(mapa_shared(acc_empty_bar(acc), 0));
       }
       if (++acc == NACC) { acc = 0; acc_phase ^= 1u; }
-      if (!any) continue;
-      if constexpr (MODE == kGated) {
-        if (mine) {
-          const int64_t sf_row = (static_cast<int64_t>(tile.first >> 7) + tile.group) * 128 + row - tile.first;
-          if (p.fp16) gated_blocks<F16Tag>(p, v, alpha, tile.group, row, sf_row, tile.tn * (BN / 2) + part * 32);
-          else gated_blocks<BF16Tag>(p, v, alpha, tile.group, row, sf_row, tile.tn * (BN / 2) + part * 32);
-        }
-        continue;
-      }
-      // The TMA clips rows behind the last row and columns behind N, but knows nothing of groups.
-      const bool by_tma = TMA_OUT > 0 && (row0 + 32 <= tile.last || tile.last == p.rows);
-      const int left = p.N - col0;
-#pragma unroll
-      for (int i = 0; i < kCols; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
-      if (bias) {
-        if (p.fp16) add_bias<F16Tag, kCols>(bias, left, v);
-        else add_bias<BF16Tag, kCols>(bias, left, v);
-      }
-      if (p.act != B2_ACT_NONE) activate<kCols>(p.act, v);
-      if (TMA_OUT > 0 && p.residual) {
+    };
+    auto sf_row_of = [&](const Part& w) {
+      return (static_cast<int64_t>(w.tile.first >> 7) + w.tile.group) * 128 + w.row - w.tile.first;
+    };
+
+    // A tile that stays in tensor memory while the epilogue loops over 16 columns at a time: nothing waits for the
+    // accumulator (there is another, or no further tile), and few registers are needed: the rolled loop took grouped
+    // products of one wave from 9.7 to 8.5 us (777 rows of 7, N = 1352, K = 1088), decode ones from 40 to 38.
+    auto hold_tile = [&](int t) {
+      const Part w = part_of(t);
+      // All 32 rows at once: in the warp's two buffers, or, where it has one, in the ring, whose last products are done
+      // when this tile's accumulator is (row-strided stores of a last tile took 4 us for 1).
+      const bool staged = whole(w);
+      const bool res_staged = staged && p.residual;
+      const uint32_t buffers = kBufs == 2 ? staging : smem_base + static_cast<uint32_t>(warp - kWarpEpi0) * 4096u;
+      static_assert(TMA_OUT == 0 || kBufs == 2 || 4 * PARTS * 4096 <= STAGES * L::kStageBytes, "buffers in the ring");
+      auto request_residual = [&] {
         if constexpr (TMA_OUT > 0) {
-          bool landed = true;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t here = staging + static_cast<uint32_t>(kBufs > 1 ? h : 0) * 2048u + (lane & 15) * 128u;
-            if (h >= kBufs && lane == 0) {
-              bulk_wait_read<0>();  // the first half's store has read the buffer
-              mbar_expect_tx(res_bar, 2048u);
-              tma_load_2d<1>(staging, &map_r, col0, row0 + 16, res_bar);
+          mbar_expect_tx(res_bar, 4096u);
+          tma_load_2d<1>(buffers, &map_r, w.col0, w.row0, res_bar);
+          tma_load_2d<1>(buffers + 2048u, &map_r, w.col0, w.row0 + 16, res_bar);
+        }
+      };
+      if constexpr (TMA_OUT > 0) {
+        if (res_staged && w.any && lane == 0) {
+          if (kBufs == 2) {
+            bulk_wait_read<0>();  // the stores of the last tile have read the buffers
+            request_residual();
+          } else {
+            tma_prefetch_2d(&map_r, w.col0, w.row0);
+            tma_prefetch_2d(&map_r, w.col0, w.row0 + 16);
+          }
+        }
+      }
+      const uint16_t* direct = p.residual && !res_staged && w.mine ? p.residual + w.at : nullptr;
+      uint4 next[2];  // the residual's 16 columns of the next step
+      if (direct) load_next(direct, p.N - w.col0, next);
+      if (!warp_wait(acc_full_bar(acc), acc_phase, 4u)) return false;
+      tc_fence_after();
+      if (w.any) {
+        if (TMA_OUT > 0 && staged) {
+          if (res_staged) {
+            if (kBufs == 1 && lane == 0) request_residual();
+            if (!warp_wait(res_bar, res_phase, 6u)) return false;
+            res_phase ^= 1u;
+          } else {
+            if (lane == 0) bulk_wait_read<0>();
+            __syncwarp();
+          }
+        }
+        const uint32_t acc_tmem = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * MMAS * BN);
+        const uint32_t here = buffers + static_cast<uint32_t>(lane >> 4) * 2048u + (lane & 15) * 128u;
+        const float gs = MODE == kGated ? __ldg(p.gs + w.tile.group) : 0.0f;
+#pragma unroll 1
+        for (int c0 = 0; c0 < (MODE == kGated ? 32 : kCols); c0 += 16) {
+          uint32_t v[16];
+          if constexpr (MODE == kGated) {
+            uint32_t up[16];
+            tmem_ld_32x16(acc_tmem + part * 32 + c0, v);
+            tmem_ld_32x16(acc_tmem + BN / 2 + part * 32 + c0, up);
+            tmem_ld_wait();
+            if (w.mine) {
+              const int col = w.tile.tn * (BN / 2) + part * 32 + c0;
+              uint32_t sf_byte;
+              uint2 packed;
+              if (p.fp16) gated_block<F16Tag>(v, up, w.alpha, gs, sf_byte, packed);
+              else gated_block<BF16Tag>(v, up, w.alpha, gs, sf_byte, packed);
+              p.sf_out[gated_sf_offset(sf_row_of(w), col, p.N / 2)] = static_cast<uint8_t>(sf_byte);
+              *reinterpret_cast<uint2*>(p.out4 + static_cast<int64_t>(w.row) * (p.N / 4) + col / 2) = packed;
             }
-            landed = warp_wait(res_bar, res_phase, 6u);
-            if (!landed) break;
-            if (kBufs == 1 || h == 1) res_phase ^= 1u;
-            if ((lane >> 4) == h) {
+            continue;
+          }
+          tmem_ld_32x16(acc_tmem + part * kCols + c0, v);
+          if (MMAS == 2 && two) {
+            uint32_t second[16];
+            tmem_ld_32x16(acc_tmem + BN + part * kCols + c0, second);
+            tmem_ld_wait();
 #pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const uint32_t at_j = here + ((static_cast<uint32_t>(j) ^ (lane & 7u)) * 16u);
-                uint32_t* o = v + 8 * j;
-                if (p.fp16) {
-                  add8<F16Tag>(lds128_vec(at_j), o);
-                  pack<F16Tag, 8>(o);
-                } else {
-                  add8<BF16Tag>(lds128_vec(at_j), o);
-                  pack<BF16Tag, 8>(o);
+            for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) + __uint_as_float(second[i]));
+          } else {
+            tmem_ld_wait();
+          }
+          const int left = p.N - w.col0 - c0;
+          if (left <= 0) break;  // the same in the whole warp
+          uint4 r[2] = {next[0], next[1]};
+          if (direct && c0 + 16 < kCols) load_next(direct + c0 + 16, left - 16, next);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * w.alpha);
+          if (w.bias) {
+            if (p.fp16) add_bias<F16Tag, 16>(w.bias + c0, left, v);
+            else add_bias<BF16Tag, 16>(w.bias + c0, left, v);
+          }
+          if (p.act != B2_ACT_NONE) activate<16>(p.act, v);
+          const uint32_t at0 = here + (((static_cast<uint32_t>(c0) >> 3) ^ (lane & 7u)) * 16u);
+          const uint32_t at1 = here + ((((static_cast<uint32_t>(c0) >> 3) + 1u) ^ (lane & 7u)) * 16u);
+          if (TMA_OUT > 0 && res_staged) {
+            r[0] = lds128_vec(at0);
+            r[1] = lds128_vec(at1);
+          }
+          if (p.residual) {  // lanes without a row add whatever lies in r and store nothing
+            if (p.fp16) {
+              add8<F16Tag>(r[0], v);
+              add8<F16Tag>(r[1], v + 8);
+            } else {
+              add8<BF16Tag>(r[0], v);
+              add8<BF16Tag>(r[1], v + 8);
+            }
+          }
+          if (p.fp16) pack<F16Tag, 16>(v);
+          else pack<BF16Tag, 16>(v);
+          if (TMA_OUT > 0 && staged) {
+            sts128(at0, v[0], v[1], v[2], v[3]);
+            sts128(at1, v[4], v[5], v[6], v[7]);
+          } else if (w.mine) {
+            uint4* dst = reinterpret_cast<uint4*>(p.D + w.at + c0);
+            dst[0] = make_uint4(v[0], v[1], v[2], v[3]);
+            if (left > 8) dst[1] = make_uint4(v[4], v[5], v[6], v[7]);
+          }
+        }
+      }
+      give_back();
+      if constexpr (TMA_OUT > 0) {
+        if (staged && w.any) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              if (w.row0 + 16 * h < p.rows) tma_store_2d(&map_d, buffers + h * 2048u, w.col0, w.row0 + 16 * h, store_policy);
+            bulk_commit();
+          }
+        }
+      }
+      return true;
+    };
+
+    // A tile whose accumulator the next products wait for (the 256 x 256 pairs): everything into registers as raw fp32,
+    // the accumulator handed back, then the same steps beside the next tile's products.
+    auto pass_tile = [&](int t) {
+      const Part w = part_of(t);
+      const bool by_tma = whole(w);
+      if constexpr (TMA_OUT > 0) {
+        // The residual (dense products only, which are always stored by the TMA) comes into the staging buffer half of the
+        // rows at a time; row-strided loads of it took 8192 x 8192 x 8192 from 199 to 277 us.
+        if (w.any && p.residual && lane == 0) {
+          bulk_wait_read<0>();  // the stores of the last tile have read the buffer
+          mbar_expect_tx(res_bar, 2048u);
+          tma_load_2d<1>(staging, &map_r, w.col0, w.row0, res_bar);
+          tma_prefetch_2d(&map_r, w.col0, w.row0 + 16);
+        }
+      }
+      if (!warp_wait(acc_full_bar(acc), acc_phase, 4u)) return false;
+      tc_fence_after();
+      uint32_t v[kCols];
+      if (w.any) {
+        const uint32_t acc_tmem = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * MMAS * BN);
+#pragma unroll
+        for (int c0 = 0; c0 < kCols; c0 += 32)
+          tmem_ld_32x32(acc_tmem + (MODE == kGated ? part * 32 + c0 / 32 * (BN / 2) : part * kCols + c0),
+                        *reinterpret_cast<uint32_t(*)[32]>(v + c0));
+        tmem_ld_wait();
+      }
+      give_back();
+      if (!w.any) return true;
+      if constexpr (MODE == kGated) {
+        if (w.mine) {
+          const float gs = __ldg(p.gs + w.tile.group);
+          const int col = w.tile.tn * (BN / 2) + part * 32;
+          uint32_t low, high;
+          uint2 first, second;
+          if (p.fp16) {
+            gated_block<F16Tag>(v, v + 32, w.alpha, gs, low, first);
+            gated_block<F16Tag>(v + 16, v + 48, w.alpha, gs, high, second);
+          } else {
+            gated_block<BF16Tag>(v, v + 32, w.alpha, gs, low, first);
+            gated_block<BF16Tag>(v + 16, v + 48, w.alpha, gs, high, second);
+          }
+          *reinterpret_cast<uint16_t*>(p.sf_out + gated_sf_offset(sf_row_of(w), col, p.N / 2)) =
+              static_cast<uint16_t>(low | high << 8);
+          *reinterpret_cast<uint4*>(p.out4 + static_cast<int64_t>(w.row) * (p.N / 4) + col / 2) =
+              make_uint4(first.x, first.y, second.x, second.y);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * w.alpha);
+        if (w.bias) {
+          if (p.fp16) add_bias<F16Tag, kCols>(w.bias, p.N - w.col0, v);
+          else add_bias<BF16Tag, kCols>(w.bias, p.N - w.col0, v);
+        }
+        if (p.act != B2_ACT_NONE) activate<kCols>(p.act, v);
+        if constexpr (TMA_OUT > 0) {
+          if (p.residual) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (h == 1 && lane == 0) {
+                bulk_wait_read<0>();  // the first half's store has read the buffer
+                mbar_expect_tx(res_bar, 2048u);
+                tma_load_2d<1>(staging, &map_r, w.col0, w.row0 + 16, res_bar);
+              }
+              if (!warp_wait(res_bar, res_phase, 6u)) return false;
+              res_phase ^= 1u;
+              if ((lane >> 4) == h) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                  const uint32_t at_j = staging + (lane & 15) * 128u + ((static_cast<uint32_t>(j) ^ (lane & 7u)) * 16u);
+                  uint32_t* o = v + 8 * j;
+                  if (p.fp16) {
+                    add8<F16Tag>(lds128_vec(at_j), o);
+                    pack<F16Tag, 8>(o);
+                  } else {
+                    add8<BF16Tag>(lds128_vec(at_j), o);
+                    pack<BF16Tag, 8>(o);
+                  }
+                  sts128(at_j, o[0], o[1], o[2], o[3]);
                 }
-                sts128(at_j, o[0], o[1], o[2], o[3]);
+              }
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) {
+                if (w.row0 + 16 * h < p.rows) tma_store_2d(&map_d, staging, w.col0, w.row0 + 16 * h, store_policy);
+                bulk_commit();
               }
             }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-              if (row0 + 16 * h < p.rows)
-                tma_store_2d(&map_d, staging + static_cast<uint32_t>(kBufs > 1 ? h : 0) * 2048u, col0, row0 + 16 * h, store_policy);
-              bulk_commit();
-            }
-          }
-          if (!landed) break;
-        }
-        continue;
-      }
-      if (residual) {
-#pragma unroll
-        for (int c = 0; c < kCols / 8; ++c) {
-          if (8 * c < left) {
-            const uint4 r = kCols == 32 ? early[c % 4] : load_residual(residual + 8 * c);
-            if (p.fp16) add8<F16Tag>(r, v + 8 * c);
-            else add8<BF16Tag>(r, v + 8 * c);
+            return true;
           }
         }
-      }
-      if (p.fp16) pack<F16Tag, kCols>(v);
-      else pack<BF16Tag, kCols>(v);
-      if (TMA_OUT > 0 && by_tma) {
-        if constexpr (TMA_OUT > 0) {
+        if (p.fp16) pack<F16Tag, kCols>(v);
+        else pack<BF16Tag, kCols>(v);
+        if (TMA_OUT > 0 && by_tma) {
+          if constexpr (TMA_OUT > 0) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {  // 16 rows at a time, in a buffer of their own where there are two
-            const uint32_t to = staging + static_cast<uint32_t>(kBufs > 1 ? h : 0) * 2048u;
-            if (lane == 0) bulk_wait_read<kBufs - 1>();  // the store that used this buffer last has read it
-            __syncwarp();
-            if ((lane >> 4) == h) {
+            for (int h = 0; h < 2; ++h) {  // 16 rows at a time
+              if (lane == 0) bulk_wait_read<0>();  // the store that used the buffer last has read it
+              __syncwarp();
+              if ((lane >> 4) == h) {
 #pragma unroll
-              for (int j = 0; j < 8; ++j)
-                sts128(to + (lane & 15) * 128u + ((static_cast<uint32_t>(j) ^ (lane & 7u)) * 16u), v[4 * j], v[4 * j + 1],
-                       v[4 * j + 2], v[4 * j + 3]);
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-              if (row0 + 16 * h < p.rows) tma_store_2d(&map_d, to, col0, row0 + 16 * h, store_policy);
-              bulk_commit();
+                for (int j = 0; j < 8; ++j)
+                  sts128(staging + (lane & 15) * 128u + ((static_cast<uint32_t>(j) ^ (lane & 7u)) * 16u), v[4 * j], v[4 * j + 1],
+                         v[4 * j + 2], v[4 * j + 3]);
+              }
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) {
+                if (w.row0 + 16 * h < p.rows) tma_store_2d(&map_d, staging, w.col0, w.row0 + 16 * h, store_policy);
+                bulk_commit();
+              }
             }
           }
-        }
-      } else if (mine) {
-        uint4* dst = reinterpret_cast<uint4*>(p.D + at);
+        } else if (w.mine) {
+          uint4* dst = reinterpret_cast<uint4*>(p.D + w.at);
 #pragma unroll
-        for (int j = 0; j < kCols / 8; ++j)
-          if (col0 + 8 * j < p.N) dst[j] = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+          for (int j = 0; j < kCols / 8; ++j)
+            if (w.col0 + 8 * j < p.N) dst[j] = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+        }
       }
-    }
+      return true;
+    };
+
+    int t = unit;
+    bool alive = true;
+    if constexpr (!kAlwaysHold)
+      for (; alive && t + num_units < num_tiles; t += num_units) alive = pass_tile(t);
+    for (; alive && t < num_tiles; t += num_units) alive = hold_tile(t);
     if constexpr (TMA_OUT > 0) {
-      if (lane == 0) bulk_wait_all();  // every store has left shared memory and is written
+      if (lane == 0) bulk_wait_read<0>();  // every store has left shared memory; the end of the grid waits for the writes
     }
   }
 
@@ -918,17 +1044,18 @@ std::atomic<int> g_grouped_variant{-1};  // test hook: -1 = automatic
 
 // The kernel for `rows` rows in `groups` groups (numbering of b2_nvfp4_grouped_gemm_set_variant).  Times on B200, back
 // to back launches from a CUDA graph, us:
-//   dense     32 x 64, 2 MMA warps   all of N in one wave of 64-wide tiles: 16 x 8192 x 8192 9.9 (32 x 128: 12.6)
-//             32 x 128               more: 16 x 28672 x 8192 26.8 (32 x 64: 31.9)
-//             128 x 64, 2 MMA warps  one wave of them: 1024^3 4.8 (256 x 128: 5.8), 200 x 4096 x 4096 7.1 (8.0)
-//             128 x 128              more columns, at most 128 rows: 64 x 28672 x 8192 29.1 (256 x 256: 31.4)
-//             256 x 128              one wave of them: 256 x 8192 x 8192 11.2 (256 x 256: 15.0, 128 x 128: 14.4)
-//             256 x 256              the rest: 2048 x 4096 x 4096 18.1 (256 x 128: 19.9)
-//   grouped   32 x 128               mean of 16 rows: 1024 rows of 64, N=2048, K=4096 60.2 (128 x 128: 61.4); 8 rows 11.9 (15.1)
-//             128 x 128              mean of 64 rows: 4096 of 64, N=K=2048 39.3 (256 x 256: 41.8), or about one wave of
-//                                    them: 777 of 7, N=1352, K=1088 8.2 (9.4)
-//             256 x 128              at most two waves of 256 x 256: 1024 of 8, N=K=2048 10.6 (256 x 256: 13.5, 128 x 128: 13.1)
-//             256 x 256              the rest: 16384 of 32, N=2816, K=2048 68.4 (256 x 128: 78.9)
+//   dense     32 x 64, 2 MMA warps   all of N in one wave of 64-wide tiles: 16 x 8192 x 8192 10.4 (32 x 128: 12.4)
+//             32 x 128               more: 16 x 28672 x 8192 25.8 (32 x 64: 35.5)
+//             128 x 64, 2 MMA warps  one wave of them: 1024^3 4.8 (128 x 128: 6.0, 256 x 128: 6.1), 200 x 4096 x 4096 7.1 (9.0, 8.4)
+//             128 x 128              more columns, at most 128 rows: 64 x 28672 x 8192 28.1 (256 x 256: 32.3)
+//             256 x 128              one wave of them: 256 x 8192 x 8192 12.1 (256 x 256: 16.2, 128 x 128: 13.5)
+//             256 x 256              the rest: 2048 x 4096 x 4096 19.3 (256 x 128: 20.4)
+//   grouped   32 x 128               mean of 16 rows: 1024 rows of 64, N=2048, K=4096 56.5 (128 x 128: 60.2); 8 rows,
+//                                    N=4096, K=2048 11.1 (14.7)
+//             128 x 128              mean of 64 rows: 4096 of 64, N=K=2048 36.9 (256 x 256: 41.8), or about one wave of
+//                                    them: 777 of 7, N=1352, K=1088 7.8 (9.4)
+//             256 x 128              at most two waves of 256 x 256: 1024 of 8, N=K=2048 10.6 (256 x 256: 14.3, 128 x 128: 11.5)
+//             256 x 256              the rest: 16384 of 32, N=2816, K=2048 67.6 (256 x 128: 73.7)
 int choose_grouped_variant(int rows, int groups, bool grouped, int N, int sms) {
   const int64_t n64 = (N + 63) / 64, n128 = (N + 127) / 128, n256 = (N + 255) / 256;
   if (!grouped) {
@@ -952,7 +1079,7 @@ int run_dense(int variant, const GroupedCall& c, cudaStream_t s) {
     case 0: return launch_grouped<kDense, 1, 64, 11, 0, 32, 2, 1>(c, s);
     case 1: return launch_grouped<kDense, 1, 128, 8, 0, 32, 1, 2>(c, s);
     case 2: return launch_grouped<kDense, 1, 64, 7, 0, 128, 2, 1>(c, s);
-    case 3: return launch_grouped<kDense, 1, 128, 6, 0, 128, 1, 2>(c, s);
+    case 3: return launch_grouped<kDense, 1, 128, 5, 1, 128, 1, 2>(c, s);
     case 4: return launch_grouped<kDense, 2, 256, 5, 1, 128, 1, 1, 1, 4>(c, s);
     default: return launch_grouped<kDense, 2, 128, 6, 1, 128, 1, 2>(c, s);
   }
@@ -962,7 +1089,7 @@ int run_groups(int variant, const GroupedCall& c, cudaStream_t s) {
     case 0:
     case 1: return launch_grouped<kGrouped, 1, 128, 8, 0, 32, 1, 2>(c, s);
     case 2:
-    case 3: return launch_grouped<kGrouped, 1, 128, 6, 0, 128, 1, 2>(c, s);
+    case 3: return launch_grouped<kGrouped, 1, 128, 5, 1, 128, 1, 2>(c, s);
     case 4: return launch_grouped<kGrouped, 2, 256, 5, 1, 128, 1, 1, 1, 4>(c, s);
     default: return launch_grouped<kGrouped, 2, 128, 6, 1, 128, 1, 2>(c, s);
   }
