@@ -1,5 +1,7 @@
 """GPU parity of the feed-forward operators: every module's own configurations against its 64-bit formula."""
 
+import dataclasses
+
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -464,6 +466,37 @@ def test_expert_ffn_captured_replayed_and_on_two_streams():
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(o, expect[i]) for o in got[i])
+
+
+@pytest.mark.parametrize("tokens,topk,experts,hidden,inner", [(1, 8, 64, 1024, 256), (3, 2, 8, 512, 192), (128, 4, 16, 512, 256), (700, 4, 40, 256, 128)])
+def test_expert_ffn_weights_and_routing_written_just_before(tokens, topk, experts, hidden, inner):
+    """The products read weights and routing ahead of the launch in front of them, but never ahead of the call."""
+    from tirx_kernels.basic import moe_ffn
+
+    x, ids, gates, weights = moe_ffn.prepare_data(tokens, topk, experts, hidden, inner)
+    first = [x, ids, gates] + [getattr(weights, f.name) for f in dataclasses.fields(weights)]
+    second = [x.flip(1), experts - 1 - ids, gates.flip(1)] + [t.flip(0) for t in first[3:]]  # other rows, experts and weights
+    sets = [first, [t.contiguous() for t in second]]
+    want = [moe_ffn.expert_ffn(*s[:3], moe_ffn.ExpertWeights(*s[3:])) for s in sets]
+    assert not torch.equal(*want)
+    live = [t.clone() for t in first]
+    live_weights = moe_ffn.ExpertWeights(*live[3:])
+
+    def turn(i):
+        for to, new in zip(live, sets[i]):
+            to.copy_(new)
+        return moe_ffn.expert_ffn(*live[:3], live_weights)
+
+    for _ in range(15):
+        for i in range(2):
+            assert torch.equal(turn(i), want[i])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = [turn(i % 2) for i in range(6)]
+    for _ in range(5):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, want[i % 2]) for i, o in enumerate(outs))
 
 
 def test_linear_and_norm_captured_and_replayed():

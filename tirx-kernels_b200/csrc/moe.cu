@@ -14,6 +14,15 @@
 #include "quant_block.cuh"
 
 namespace b2 {
+
+// nvfp4_grouped_gemm.cu
+int grouped_product(const void* A, const void* B, const void* SFA, const void* SFB, const float* alpha_dev,
+                    const int32_t* offsets_dev, const void* bias, void* D, int rows, int groups, int N, int K,
+                    int out_dtype, int activation, bool early, const int32_t* ids_dev, void* stream);
+int grouped_product_gated(const void* A, const void* B, const void* SFA, const void* SFB, const float* alpha_dev,
+                          const int32_t* offsets_dev, const float* gs_dev, void* out, void* sf, int rows, int groups,
+                          int inner, int K, int dtype, bool early, const int32_t* ids_dev, void* stream);
+
 namespace {
 
 constexpr int kMaxGroups = 384;  // as in nvfp4_grouped_gemm.cu
@@ -747,20 +756,23 @@ extern "C" int b2_moe_expert_ffn(const void* x, const int32_t* ids_dev, const fl
   if (int rc = b2_moe_dispatch(x, ids_dev, gs1_dev, offsets, row_token, position, base + w.a1, base + w.sf1, tokens, topk,
                                experts, hidden, dtype, stream))
     return rc;
+  // Both products read early: weights and ids were there before the dispatch, the offsets before the launch in front of
+  // the product, but for those that the dispatch itself writes.  There the first product counts the ids.
+  const int32_t* counted = rows <= kPlanInDispatch ? ids_dev : nullptr;
   if (inner % 128 == 0) {
-    if (int rc = b2_nvfp4_grouped_gemm_gated(base + w.a1, W1, base + w.sf1, SF1, alpha1_dev, offsets, gs2_dev, base + w.a2,
-                                             base + w.sf2, rows, experts, inner, hidden, dtype, stream))
+    if (int rc = grouped_product_gated(base + w.a1, W1, base + w.sf1, SF1, alpha1_dev, offsets, gs2_dev, base + w.a2,
+                                       base + w.sf2, rows, experts, inner, hidden, dtype, true, counted, stream))
       return rc;
   } else {
-    if (int rc = b2_nvfp4_grouped_gemm(base + w.a1, W1, base + w.sf1, SF1, alpha1_dev, offsets, nullptr, base + w.y1, rows,
-                                       experts, 2 * inner, hidden, dtype, B2_ACT_NONE, stream))
+    if (int rc = grouped_product(base + w.a1, W1, base + w.sf1, SF1, alpha1_dev, offsets, nullptr, base + w.y1, rows, experts,
+                                 2 * inner, hidden, dtype, B2_ACT_NONE, true, counted, stream))
       return rc;
     if (int rc = b2_nvfp4_quantize_grouped(base + w.y1, nullptr, offsets, base + w.a2, base + w.sf2, gs2_dev, rows, rows,
                                            experts, inner, dtype, 1, stream))
       return rc;
   }
-  if (int rc = b2_nvfp4_grouped_gemm(base + w.a2, W2, base + w.sf2, SF2, alpha2_dev, offsets, nullptr, base + w.z, rows,
-                                     experts, hidden, inner, dtype, B2_ACT_NONE, stream))
+  if (int rc = grouped_product(base + w.a2, W2, base + w.sf2, SF2, alpha2_dev, offsets, nullptr, base + w.z, rows, experts,
+                               hidden, inner, dtype, B2_ACT_NONE, true, nullptr, stream))
     return rc;
   return b2_moe_combine(base + w.z, position, weight_dev, residual, out, rows, tokens, topk, hidden, dtype, stream);
 }

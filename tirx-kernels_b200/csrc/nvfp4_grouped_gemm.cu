@@ -26,6 +26,7 @@
 //     or a CTA has one tile, it loops over 16 columns of the held one.  The 256 x 256 pair has room for one: 16
 //     epilogue warps take it into registers as raw fp32 (64 columns a thread; 8 warps would need 128, hence setmaxnreg)
 //     and hand it back before they compute anything; the last tile, which nothing waits for, is held again.
+#include <algorithm>
 #include <atomic>
 
 #include "nvfp4_tile.cuh"
@@ -52,6 +53,10 @@ struct GroupedParams {
   int act;                  // B2_ACT_*
   int fp16;                 // 16-bit type of bias, residual and D
   uint64_t wait_budget_ns;
+  // The routed feed-forward's calls (single-CTA tiles): weights and the list of groups were there before the launch in
+  // front of this one began, and are read while it runs.
+  int early;
+  const int32_t* ids;       // [rows] groups of the rows, in any order, to be counted instead of `offsets`, or null
   // kGated: the weight is [gate rows | up rows] of N / 2 each, and SiLU(gate) * up leaves quantized
   const float* gs;          // [groups] encode scale of the output
   uint8_t* out4;            // [rows, N / 4] packed E2M1
@@ -338,19 +343,49 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
   if constexpr (CG == 2) cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem_base = kWarpWide ? __shfl_sync(0xffffffffu, *tmem_slot, 0) : *tmem_slot;
-  // Dependent launch as in nvfp4_gemm.cu: nothing in front of this wait touches global memory.
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  // Dependent launch as in nvfp4_gemm.cu: nothing in front of this wait touches global memory.  The exception are early
+  // calls.  Their predecessor let them start behind its own wait, so everything in front of it is complete: the table of
+  // groups and the first weights are read beside it (one token through 8 experts of 64,
+  // 4096 x 1024: 28.3 us for 29.9).
+  constexpr bool kMayBeEarly = CG == 1 && MODE != kDense;
+  const bool early = kMayBeEarly && p.early;
+  auto dependent_launch = [] {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  };
+  if (!early) dependent_launch();
   if constexpr (MODE != kDense) {
     if (warp == kGWarpMma2) {
-      int tiles = 0;  // row tiles in front of the 32 groups of this step
+      const bool counted = kMayBeEarly && p.ids;
+      if (counted) {
+        for (int g = lane; g < p.groups; g += 32) starts[g] = 0;
+        __syncwarp();
+#pragma unroll 4
+        for (int i = lane; i < p.rows; i += 32) {
+          const int id = __ldcg(p.ids + i);
+          if (id >= 0 && id < p.groups) atomicAdd(starts + id, 1);
+        }
+        __syncwarp();
+      }
+      int tiles = 0, rows = 0;  // row tiles, counted rows in front of the 32 groups of this step
       for (int g0 = 0; g0 < p.groups; g0 += 32) {
         const int g = g0 + lane;
         int first = 0, last = 0;
-        if (g < p.groups) {
+        if (counted) {
+          const int count = g < p.groups ? starts[g] : 0;
+          last = count;
+#pragma unroll
+          for (int d = 1; d < 32; d <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, last, d);
+            if (lane >= d) last += up;
+          }
+          last += rows;
+          first = last - count;
+          rows = __shfl_sync(0xffffffffu, last, 31);
+        } else if (g < p.groups) {
           // Offsets that are not ascending or leave [0, rows] are brought back into it: no access leaves A or D.
-          first = min(max(__ldg(p.offsets + g), 0), p.rows);
-          last = min(max(__ldg(p.offsets + g + 1), first), p.rows);
+          first = min(max(__ldcg(p.offsets + g), 0), p.rows);
+          last = min(max(__ldcg(p.offsets + g + 1), first), p.rows);
         }
         const int mine = (last - first + kBM - 1) / kBM;
         int sum = mine;
@@ -372,6 +407,7 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
     }
     __syncthreads();
   }
+  if (early && warp != kGWarpOperands && warp != kGWarpScales) dependent_launch();
   // What the issuing warps compute from shared memory is made uniform by a shuffle, or the compiler would keep their
   // loops' state out of uniform registers (nvfp4_gemm.cu).
   auto uniform = [](int v) { return kWarpWide ? __shfl_sync(0xffffffffu, v, 0) : v; };
@@ -398,26 +434,50 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
     if (warp == kGWarpOperands) {
       // ================= TMA producer of the operands =================
       if (kWarpWide || lane == 0) {
+        // Gated: the first half of the tile's columns are gates, the second (the pair's second CTA's) the matching ups.
+        auto first_row_b = [&](const Tile& tile) {
+          return MODE == kGated ? uniform(tile.group * p.N + tile.tn * (BN / 2)) + static_cast<int>(rank) * (p.N / 2)
+                                : uniform(tile.group * p.N + tile.tn * BN) + static_cast<int>(rank) * L::kBRows;
+        };
+        auto load_b = [&](uint32_t sbase, int ks, int row_b, uint32_t op_bar) {
+          tma_load_2d<CG>(sbase + L::kABytes, &map_b, ks * 128, row_b, op_bar);
+          if constexpr (MODE == kGated && CG == 1)
+            tma_load_2d<CG>(sbase + L::kABytes + L::kBBytes / 2, &map_b, ks * 128, row_b + p.N / 2, op_bar);
+        };
+        int ahead = 0;  // slabs whose B is on its way
+        if constexpr (kMayBeEarly) {
+          if (early) {
+            for (int t = unit; t < num_tiles && ahead < STAGES; t += num_units) {
+              const int row_b = first_row_b(find_tile<MODE>(p, starts, group_rows, t));
+              for (int ks = 0; ks < k_slabs && ahead < STAGES; ++ks, ++ahead) {
+                mbar_expect_tx(full_bar(ahead), kOperandTx);
+                load_b(smem_base + ahead * L::kStageBytes, ks, row_b, full_bar(ahead));
+              }
+            }
+            dependent_launch();
+          }
+        }
         int stage = 0;
         uint32_t phase = 0;
         bool alive = true;
         for (int t = unit; t < num_tiles && alive; t += num_units) {
           const Tile tile = find_tile<MODE>(p, starts, group_rows, t);
           const int row_a = uniform(tile.first + tile.tm * kBM) + static_cast<int>(rank) * kBlockM;
-          // Gated: the first half of the tile's columns are gates, the second (the pair's second CTA's) the matching ups.
-          const int row_b = MODE == kGated ? uniform(tile.group * p.N + tile.tn * (BN / 2)) + static_cast<int>(rank) * (p.N / 2)
-                                           : uniform(tile.group * p.N + tile.tn * BN) + static_cast<int>(rank) * L::kBRows;
+          const int row_b = first_row_b(tile);
           for (int ks = 0; ks < k_slabs; ++ks) {
             if (!role_wait(empty_bar(stage), phase ^ 1u, 1u)) { alive = false; break; }
             const uint32_t sbase = smem_base + stage * L::kStageBytes;
             // operand bytes of both CTAs of a pair are counted on the leader's barrier
             const uint32_t op_bar = CG == 2 ? mapa_shared(full_bar(stage), 0) : full_bar(stage);
             if (issues()) {
-              if (leader) mbar_expect_tx(full_bar(stage), kOperandTx);
-              tma_load_2d<CG>(sbase, &map_a, ks * 128, row_a, op_bar);
-              tma_load_2d<CG>(sbase + L::kABytes, &map_b, ks * 128, row_b, op_bar);
-              if constexpr (MODE == kGated && CG == 1)
-                tma_load_2d<CG>(sbase + L::kABytes + L::kBBytes / 2, &map_b, ks * 128, row_b + p.N / 2, op_bar);
+              if (kMayBeEarly && ahead > 0) {
+                --ahead;
+                tma_load_2d<CG>(sbase, &map_a, ks * 128, row_a, op_bar);
+              } else {
+                if (leader) mbar_expect_tx(full_bar(stage), kOperandTx);
+                tma_load_2d<CG>(sbase, &map_a, ks * 128, row_a, op_bar);
+                load_b(sbase, ks, row_b, op_bar);
+              }
             }
             if constexpr (kWarpWide) __syncwarp();
             if (++stage == STAGES) { stage = 0; phase ^= 1u; }
@@ -428,22 +488,46 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
       // ================= TMA producer of the scale factors =================
       if (kWarpWide || lane == 0) {
         const int sfb_tiles = (p.N + 127) / 128;
+        auto first_tile_b = [&](const Tile& tile) {
+          return uniform(tile.group * sfb_tiles + (tile.tn * (MODE == kGated ? BN / 2 : BN)) / 128);
+        };
+        auto load_b = [&](uint32_t sf_smem, int ks, int sfb_tile, uint32_t bar) {
+          tma_load_3d<1>(sf_smem + L::kSfaBytes, &map_sfb, 0, ks * 4, sfb_tile, bar);
+          if constexpr (MODE == kGated)
+            tma_load_3d<1>(sf_smem + L::kSfaBytes + 2048, &map_sfb, 0, ks * 4, sfb_tile + p.N / 256, bar);
+        };
+        int ahead = 0;  // slabs whose scales of B are on their way
+        if constexpr (kMayBeEarly) {
+          if (early) {
+            for (int t = unit; t < num_tiles && ahead < STAGES; t += num_units) {
+              const int sfb_tile = first_tile_b(find_tile<MODE>(p, starts, group_rows, t));
+              for (int ks = 0; ks < k_slabs && ahead < STAGES; ++ks, ++ahead) {
+                mbar_expect_tx(sfload_bar(ahead), kScaleTx);
+                load_b(smem_base + ahead * L::kStageBytes + L::kABytes + L::kBBytes, ks, sfb_tile, sfload_bar(ahead));
+              }
+            }
+            dependent_launch();
+          }
+        }
         int stage = 0;
         uint32_t phase = 0;
         bool alive = true;
         for (int t = unit; t < num_tiles && alive; t += num_units) {
           const Tile tile = find_tile<MODE>(p, starts, group_rows, t);
           const int sfa_tile = uniform((tile.first >> 7) + tile.group + ((tile.tm * kBM) >> 7)) + static_cast<int>(rank);
-          const int sfb_tile = uniform(tile.group * sfb_tiles + (tile.tn * (MODE == kGated ? BN / 2 : BN)) / 128);
+          const int sfb_tile = first_tile_b(tile);
           for (int ks = 0; ks < k_slabs; ++ks) {
             if (!role_wait(empty_bar(stage), phase ^ 1u, 1u)) { alive = false; break; }
             const uint32_t sf_smem = smem_base + stage * L::kStageBytes + L::kABytes + L::kBBytes;
             if (issues()) {
-              mbar_expect_tx(sfload_bar(stage), kScaleTx);
-              tma_load_3d<1>(sf_smem, &map_sfa, 0, ks * 4, sfa_tile, sfload_bar(stage));
-              tma_load_3d<1>(sf_smem + L::kSfaBytes, &map_sfb, 0, ks * 4, sfb_tile, sfload_bar(stage));
-              if constexpr (MODE == kGated)
-                tma_load_3d<1>(sf_smem + L::kSfaBytes + 2048, &map_sfb, 0, ks * 4, sfb_tile + p.N / 256, sfload_bar(stage));
+              if (kMayBeEarly && ahead > 0) {
+                --ahead;
+                tma_load_3d<1>(sf_smem, &map_sfa, 0, ks * 4, sfa_tile, sfload_bar(stage));
+              } else {
+                mbar_expect_tx(sfload_bar(stage), kScaleTx);
+                tma_load_3d<1>(sf_smem, &map_sfa, 0, ks * 4, sfa_tile, sfload_bar(stage));
+                load_b(sf_smem, ks, sfb_tile, sfload_bar(stage));
+              }
             }
             if constexpr (kWarpWide) __syncwarp();
             if (++stage == STAGES) { stage = 0; phase ^= 1u; }
@@ -975,9 +1059,10 @@ int launch_grouped(const GroupedCall& c, cudaStream_t stream) {
     set_error("%s: %lld tiles exceed the tile list's range", c.who, static_cast<long long>(tiles));
     return B2_ERR_INVALID_ARGUMENT;
   }
-  // As many persistent CTAs (pairs) as finish the tiles in the fewest rounds, and no more.
+  // Persistent CTAs (pairs): of a dense product as many as finish its tiles in the fewest rounds; groups may have fewer
+  // tiles than `tiles`, so all that fit (with the dense rule 16384 rows of 32 groups took 13 rounds for 12).
   const int64_t rounds = (tiles + sms / CG - 1) / (sms / CG);
-  const int units = static_cast<int>((tiles + rounds - 1) / rounds);
+  const int units = static_cast<int>(MODE == kDense ? (tiles + rounds - 1) / rounds : std::min<int64_t>(tiles, sms / CG));
 
   {
     static std::atomic<bool> configured[64] = {};  // per instantiation; setting it twice does no harm
@@ -1050,12 +1135,12 @@ std::atomic<int> g_grouped_variant{-1};  // test hook: -1 = automatic
 //             128 x 128              more columns, at most 128 rows: 64 x 28672 x 8192 28.1 (256 x 256: 32.3)
 //             256 x 128              one wave of them: 256 x 8192 x 8192 12.1 (256 x 256: 16.2, 128 x 128: 13.5)
 //             256 x 256              the rest: 2048 x 4096 x 4096 19.3 (256 x 128: 20.4)
-//   grouped   32 x 128               mean of 16 rows: 1024 rows of 64, N=2048, K=4096 56.5 (128 x 128: 60.2); 8 rows,
-//                                    N=4096, K=2048 11.1 (14.7)
-//             128 x 128              mean of 64 rows: 4096 of 64, N=K=2048 36.9 (256 x 256: 41.8), or about one wave of
-//                                    them: 777 of 7, N=1352, K=1088 7.8 (9.4)
-//             256 x 128              at most two waves of 256 x 256: 1024 of 8, N=K=2048 10.6 (256 x 256: 14.3, 128 x 128: 11.5)
-//             256 x 256              the rest: 16384 of 32, N=2816, K=2048 67.6 (256 x 128: 73.7)
+//   grouped   32 x 128               mean of 16 rows: 1024 rows of 64, N=2048, K=4096 55.3 (128 x 128: 56.1); 8 rows,
+//                                    N=4096, K=2048 11.1 (14.3)
+//             128 x 128              mean of 64 rows: 4096 of 64, N=K=2048 36.5 (256 x 256: 39.3), or about one wave of
+//                                    them: 777 of 7, N=1352, K=1088 7.4 (256 x 128: 8.6)
+//             256 x 128              at most two waves of 256 x 256: 1024 of 8, N=K=2048 10.2 (256 x 256: 11.1, 128 x 128: 11.1)
+//             256 x 256              the rest: 16384 of 32, N=2816, K=2048 65.1 (256 x 128: 73.1)
 int choose_grouped_variant(int rows, int groups, bool grouped, int N, int sms) {
   const int64_t n64 = (N + 63) / 64, n128 = (N + 127) / 128, n256 = (N + 255) / 256;
   if (!grouped) {
@@ -1185,10 +1270,12 @@ extern "C" int b2_nvfp4_gemm_epilogue(const void* A, const void* B, const void* 
   return run_grouped(c, static_cast<cudaStream_t>(stream));
 }
 
-extern "C" int b2_nvfp4_grouped_gemm(const void* A, const void* B, const void* SFA, const void* SFB,
-                                     const float* alpha_dev, const int32_t* offsets_dev, const void* bias, void* D,
-                                     int rows, int groups, int N, int K, int out_dtype, int activation, void* stream) {
-  using namespace b2;
+namespace b2 {
+
+// The grouped products; `early` and `ids` (GroupedParams) are the routed feed-forward's (moe.cu).
+int grouped_product(const void* A, const void* B, const void* SFA, const void* SFB, const float* alpha_dev,
+                    const int32_t* offsets_dev, const void* bias, void* D, int rows, int groups, int N, int K,
+                    int out_dtype, int activation, bool early, const int32_t* ids_dev, void* stream) {
   GroupedCall c = {};
   c.who = "b2_nvfp4_grouped_gemm";
   c.A = A;
@@ -1205,6 +1292,8 @@ extern "C" int b2_nvfp4_grouped_gemm(const void* A, const void* B, const void* S
   c.p.N = N;
   c.p.act = activation;
   c.p.fp16 = out_dtype == B2_DTYPE_F16;
+  c.p.early = early;
+  c.p.ids = ids_dev;
   c.p.wait_budget_ns = kWaitBudgetNs;
   if (int rc = check_product(c, out_dtype)) return rc;
   if (rows == 0) return B2_OK;
@@ -1217,11 +1306,9 @@ extern "C" int b2_nvfp4_grouped_gemm(const void* A, const void* B, const void* S
   return run_grouped(c, static_cast<cudaStream_t>(stream));
 }
 
-extern "C" int b2_nvfp4_grouped_gemm_gated(const void* A, const void* B, const void* SFA, const void* SFB,
-                                           const float* alpha_dev, const int32_t* offsets_dev, const float* gs_dev,
-                                           void* out, void* sf, int rows, int groups, int inner, int K, int dtype,
-                                           void* stream) {
-  using namespace b2;
+int grouped_product_gated(const void* A, const void* B, const void* SFA, const void* SFB, const float* alpha_dev,
+                          const int32_t* offsets_dev, const float* gs_dev, void* out, void* sf, int rows, int groups,
+                          int inner, int K, int dtype, bool early, const int32_t* ids_dev, void* stream) {
   GroupedCall c = {};
   c.who = "b2_nvfp4_grouped_gemm_gated";
   if (inner < 128 || inner % 128 != 0 || inner > (1 << 29)) {
@@ -1243,6 +1330,8 @@ extern "C" int b2_nvfp4_grouped_gemm_gated(const void* A, const void* B, const v
   c.p.N = 2 * inner;
   c.p.act = B2_ACT_NONE;
   c.p.fp16 = dtype == B2_DTYPE_F16;
+  c.p.early = early;
+  c.p.ids = ids_dev;
   c.p.wait_budget_ns = kWaitBudgetNs;
   if (int rc = check_product(c, dtype)) return rc;
   if (rows == 0) return B2_OK;
@@ -1253,6 +1342,23 @@ extern "C" int b2_nvfp4_grouped_gemm_gated(const void* A, const void* B, const v
   c.sfa_tiles = rows / 128 + groups;
   if (int rc = grouped_status_words(&c.p.status)) return rc;
   return run_grouped(c, static_cast<cudaStream_t>(stream));
+}
+
+}  // namespace b2
+
+extern "C" int b2_nvfp4_grouped_gemm(const void* A, const void* B, const void* SFA, const void* SFB,
+                                     const float* alpha_dev, const int32_t* offsets_dev, const void* bias, void* D,
+                                     int rows, int groups, int N, int K, int out_dtype, int activation, void* stream) {
+  return b2::grouped_product(A, B, SFA, SFB, alpha_dev, offsets_dev, bias, D, rows, groups, N, K, out_dtype, activation,
+                             false, nullptr, stream);
+}
+
+extern "C" int b2_nvfp4_grouped_gemm_gated(const void* A, const void* B, const void* SFA, const void* SFB,
+                                           const float* alpha_dev, const int32_t* offsets_dev, const float* gs_dev,
+                                           void* out, void* sf, int rows, int groups, int inner, int K, int dtype,
+                                           void* stream) {
+  return b2::grouped_product_gated(A, B, SFA, SFB, alpha_dev, offsets_dev, gs_dev, out, sf, rows, groups, inner, K, dtype,
+                                   false, nullptr, stream);
 }
 
 extern "C" int b2_nvfp4_grouped_gemm_set_variant(int variant) {
