@@ -6,6 +6,8 @@ A kernel module lives at ``tirx_kernels/<category>/.../<module>.py`` and exposes
     a *literal* dict assigned exactly once: ``name`` (str, the public ``--kernel`` name),
     ``category`` (str, the containing bucket directory) and ``compute_capability`` (int,
     10 for sm_100a).
+    A module of an operator that the reference's registry does not have names the same dict ``OPERATOR_META``:
+    ``registry.load_kernel`` and the CLIs find it by name, the registry's index stays the reference's.
 ``CONFIGS`` / optional ``BENCH_CONFIGS``
     lists of dicts, each with a unique ``label`` plus the keyword arguments of the module's
     functions.  The bench CLI prefers ``BENCH_CONFIGS``.
