@@ -759,7 +759,8 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
 
     // A tile that stays in tensor memory while the epilogue loops over 16 columns at a time: nothing waits for the
     // accumulator (there is another, or no further tile), and few registers are needed: the rolled loop took grouped
-    // products of one wave from 9.7 to 8.5 us (777 rows of 7, N = 1352, K = 1088), decode ones from 40 to 38.
+    // products of one wave from 9.7 to 8.5 us (777 rows of 7, N = 1352, K = 1088), decode ones from 40 to 38.  (32 columns
+    // at a time: 200 x 4096 x 4096 7.1 us for 6.4, 256 x 8192 x 8192 11.6 for 10.9.)
     auto hold_tile = [&](int t) {
       const Part w = part_of(t);
       // All 32 rows at once: in the warp's two buffers, or, where it has one, in the ring, whose last products are done
@@ -1164,8 +1165,9 @@ std::atomic<int> g_grouped_variant{-1};  // test hook: -1 = automatic
 //   dense     32 x 64, 2 MMA warps   all of N in one wave of 64-wide tiles: 16 x 8192 x 8192 10.4 (32 x 128: 12.4)
 //             32 x 128               more: 16 x 28672 x 8192 25.8 (32 x 64: 35.5)
 //             128 x 64, 2 MMA warps  one wave of them: 1024^3 4.8 (128 x 128: 6.0, 256 x 128: 6.1), 200 x 4096 x 4096 7.1 (9.0, 8.4)
-//             128 x 128              more columns, at most 128 rows: 64 x 28672 x 8192 28.1 (256 x 256: 32.3)
-//             256 x 128              one wave of them: 256 x 8192 x 8192 12.1 (256 x 256: 16.2, 128 x 128: 13.5)
+//             128 x 128              more columns, at most 128 rows: 64 x 28672 x 8192 28.1 (256 x 256: 32.3), or K up to 2048
+//                                    and one wave: 1000 x 2048 x 2048 6.1 (256 x 128: 6.7; at K = 4096 both 8.2)
+//             256 x 128              one wave of them: 256 x 8192 x 8192 10.9 (256 x 256: 16.2, 128 x 128: 12.4)
 //             256 x 256              the rest: 2048 x 4096 x 4096 19.3 (256 x 128: 20.4)
 //   grouped   32 x 128               mean of 16 rows: 1024 rows of 64, N=2048, K=4096 55.3 (128 x 128: 56.1); 8 rows,
 //                                    N=4096, K=2048 11.1 (14.3)
@@ -1173,13 +1175,13 @@ std::atomic<int> g_grouped_variant{-1};  // test hook: -1 = automatic
 //                                    them: 777 of 7, N=1352, K=1088 7.4 (256 x 128: 8.6)
 //             256 x 128              at most two waves of 256 x 256: 1024 of 8, N=K=2048 10.2 (256 x 256: 11.1, 128 x 128: 11.1)
 //             256 x 256              the rest: 16384 of 32, N=2816, K=2048 65.1 (256 x 128: 73.1)
-int choose_grouped_variant(int rows, int groups, bool grouped, int N, int sms) {
+int choose_grouped_variant(int rows, int groups, bool grouped, int N, int K, int sms) {
   const int64_t n64 = (N + 63) / 64, n128 = (N + 127) / 128, n256 = (N + 255) / 256;
   if (!grouped) {
     const int64_t m128 = (rows + 127) / 128, m256 = (rows + 255) / 256;
     if (rows <= 32) return n64 <= sms ? 0 : 1;
     if (m128 * n64 <= sms) return 2;
-    if (rows <= 128) return 3;
+    if (rows <= 128 || (K <= 2048 && m128 * n128 <= sms)) return 3;
     return m256 * n128 <= sms / 2 ? 5 : 4;
   }
   // The groups' sizes are known on the device alone: a group's last tile is taken to be half full.
@@ -1229,7 +1231,7 @@ int run_grouped(const GroupedCall& c, cudaStream_t s) {
   const int sms = device_sm_count();
   if (sms <= 0) return B2_ERR_CUDA;
   int variant = g_grouped_variant.load(std::memory_order_relaxed);
-  if (variant < 0) variant = choose_grouped_variant(c.p.rows, c.p.groups, c.p.offsets != nullptr, c.p.N, sms);
+  if (variant < 0) variant = choose_grouped_variant(c.p.rows, c.p.groups, c.p.offsets != nullptr, c.p.N, c.K, sms);
   if (c.p.out4) return run_gated(variant, c, s);
   return c.p.offsets ? run_groups(variant, c, s) : run_dense(variant, c, s);
 }
