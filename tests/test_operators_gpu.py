@@ -200,6 +200,18 @@ def test_grouped_many_groups_and_tiles(variant):
         mod.run_test(2000, 3, 4104, 64, bias=False)
 
 
+@pytest.mark.parametrize("which", [1, 3, 4])
+def test_grouped_more_row_tiles_than_are_mapped(which, variant):
+    """Behind the row tiles whose group is looked up (512 of single CTAs, 128 of pairs) it is searched."""
+    from tirx_kernels.basic import nvfp4_grouped_gemm as mod
+
+    variant(which)
+    mod.run_test(70000 if which == 3 else 20000, 300, 136, 64, bias=False)
+    sizes = [0] * 384
+    sizes[0], sizes[200], sizes[383] = 40000, 1, 39000
+    mod.run_test(79001, 384, 72, 64, bias=False, sizes=sizes)
+
+
 def test_grouped_leaves_other_rows_alone():
     """Rows in front of offsets[0] and behind offsets[groups] keep their bytes, in every tile they share with a group."""
     from tirx_kernels import _checks, _native
