@@ -274,3 +274,33 @@ def test_every_operator_argument_list_matches_the_header():
         count = 0 if declared.strip() in ("", "void") else declared.count(",") + 1
         assert count == len(_native.MAIN_SIGNATURES[name][1]), name
     assert ctypes.sizeof(ctypes.c_void_p) == 8
+
+
+def test_bound_calls_refuse_what_they_are_not_made_for():
+    """The compiled half of a call: counts and kinds when it is bound, tensors and counts when it is called; nothing is launched."""
+    from tirx_kernels import _checks, _native
+
+    bind = _native._binding().bind
+    spec = _checks.tensor_spec
+    specs = tuple(spec(n, "uint8", -1) for n in ("A", "B", "SFA", "SFB")) + (spec("alpha", "float32", 1), spec("bias", "bfloat16", (8,), True),
+                                                                              spec("residual", "bfloat16", (4, 8), True), spec("D", "bfloat16", (4, 8)))
+    for symbol, address, some, sizes in [("b2_nvfp4_gemm", 1, specs, (1,) * 5), ("b2_nvfp4_gemm_epilogue", 0, specs, (1,) * 5),
+                                         ("b2_nvfp4_gemm_epilogue", 1, specs[:7], (1,) * 5), ("b2_nvfp4_gemm_epilogue", 1, specs, (1,) * 4),
+                                         ("b2_nvfp4_gemm_epilogue", 1, specs, (1, 1, 1, 1, 0.5)), (None, 0, specs, (1,)), (None, 0, specs * 3, ()),
+                                         (None, 0, (("A", "uint8", 1, False),), ()), (None, 0, (("A", torch.uint8, "x", False),), ()),
+                                         (None, 0, [], ())]:
+        with pytest.raises(TypeError):
+            bind(symbol, address, some, sizes)
+    check = bind(None, 0, (spec("a", "float32", (2, 3)), spec("b", "int32", 4, True)), ())
+    a = torch.zeros(2, 3)
+    for tensors in [(a, None), (None, None), (1, None), ("a", None), (a.double(), None), (torch.empty(2, 3, device="meta"), None),
+                    (a, torch.zeros(4, dtype=torch.int32))]:
+        assert check(*tensors) == -1
+    assert bind(None, 0, (spec("b", "int32", 4, True),), ())(None) == 0
+    for arguments in [(), (a,), (a, None, None)]:
+        with pytest.raises(TypeError):
+            check(*arguments)
+    with pytest.raises(TypeError):
+        check(a, b=None)
+    with pytest.raises(ValueError, match="a: all tensors must be CUDA"):
+        _native.Launch(None, (spec("a", "float32", (2, 3)),))(a)

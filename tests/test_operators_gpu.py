@@ -665,3 +665,36 @@ def test_a_block_of_them_together(tokens):
     _near(h, want_h, 2.0**-8 * want_h.abs() + 2e-6 * (want_h.abs() + 2 * down.double().abs()) + 1e-7)
     torch.cuda.synchronize()
     _native.nvfp4_grouped_gemm_status()
+
+
+def test_bound_calls_check_every_tensor_and_follow_stream_and_numbers():
+    """The compiled check agrees with the spelled-out one; a given number that is none raises; the current stream is used."""
+    from tirx_kernels import _checks, _native
+    from tirx_kernels.basic import gated_add_rmsnorm_fp4quant as norm
+
+    spec = _checks.tensor_spec
+    check = _native.Launch(None, (spec("a", "float32", (2, 3)), spec("b", "uint8", -1, True)))
+    a = torch.zeros(2, 3, device="cuda")
+    check(a, None), check(a, torch.zeros(0, dtype=torch.uint8, device="cuda")), check(torch.nn.Parameter(a), None)
+    for tensors, message in [((a.t().contiguous().t(), None), "contiguous"), ((a.half(), None), "a must be torch.float32"),
+                             ((a.view(3, 2), None), "shape"), ((a, a.byte().cpu()), "b: all tensors must be CUDA"), ((None, None), "a must be a tensor")]:
+        with pytest.raises(ValueError, match=message):
+            check(*tensors)
+    x, residual, w_post, gate, w_pre, _ = norm.prepare_data("bfloat16", 6, 256)
+    ex = _launcher(norm, input_dtype="bfloat16", M=6, H=256, quantize=False)
+    h, y = torch.empty_like(x), torch.empty_like(x)
+    with pytest.raises(TypeError):
+        ex(x, residual, w_post, gate, w_pre, h, y, None, None, "0.9", 1e-6)
+    ex(x, residual, w_post, gate, w_pre, h, y, None, None, 1, 1e-6)  # an integer is a number too
+    want = h.clone()
+    ex(x, residual, w_post, gate, w_pre, h, y, None, None, 1.0, 1e-6)
+    assert torch.equal(h, want)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        late = torch.empty_like(x)
+        torch.cuda._sleep(2_000_000)
+        late.copy_(x)
+        ex(late, residual, w_post, gate, w_pre, h, y, None, None, 1.0, 1e-6)  # behind the copy, on its stream
+    stream.synchronize()
+    assert torch.equal(h, want)

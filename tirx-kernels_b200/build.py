@@ -5,6 +5,7 @@
 Outputs (git-ignored, next to this file):
     lib/libb200nvfp4.so           quantizers, GEMM, probe  (the product; no cuBLAS dependency)
     lib/libb200nvfp4_cublaslt.so  cuBLASLt NVFP4 baseline   (library peer used only by benches)
+    lib/b200nvfp4_binding.so      the operators' calls from Python (a CPython module on PyTorch's tensor interface)
 
 nvcc cross-compiles without a GPU, so this runs on a CPU-only machine.
 """
@@ -80,8 +81,23 @@ def _link(objs: list[Path], out: Path, extra: list[str], force: bool, verbose: b
     _run(cmd, verbose, out.stem)
 
 
+def _binding(force: bool, verbose: bool) -> Path:
+    import sysconfig
+
+    from torch.utils.cpp_extension import include_paths, library_paths
+
+    src, out = CSRC / "binding.cpp", LIB / "b200nvfp4_binding.so"
+    newest = max(src.stat().st_mtime, (INCLUDE / "b200_nvfp4.h").stat().st_mtime, Path(__file__).stat().st_mtime)
+    if not force and out.exists() and out.stat().st_mtime >= newest:
+        return out
+    includes = [str(INCLUDE), sysconfig.get_paths()["include"], *include_paths("cuda")]
+    _run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", *(f"-I{p}" for p in includes), str(src), "-o", str(out),
+          *(f"-L{p}" for p in library_paths("cuda")), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"], verbose, "binding")
+    return out
+
+
 def build(force: bool = False, verbose: bool = False) -> dict[str, Path]:
-    """Compile every CUDA source for sm_100a and link both shared libraries."""
+    """Compile every CUDA source for sm_100a and link the shared libraries."""
     built: dict[str, Path] = {}
     main_objs = [_compile(CSRC / s, force, verbose) for s in MAIN_SOURCES if (CSRC / s).exists()]
     main = LIB / "libb200nvfp4.so"
@@ -94,6 +110,7 @@ def build(force: bool = False, verbose: bool = False) -> dict[str, Path]:
         cuda_home = os.environ.get("CUDA_HOME", "/usr/local/cuda")
         _link(lt_objs, lt, ["-cudart", "static", f"-L{cuda_home}/lib64", "-lcublasLt"], force, verbose)
         built["cublaslt"] = lt
+    built["binding"] = _binding(force, verbose)
     return built
 
 

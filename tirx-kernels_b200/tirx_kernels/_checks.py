@@ -106,7 +106,8 @@ def dequantized_matmul_fp32(A_fp4, B_fp4, A_sf, B_sf, alpha: float, *, row_chunk
 
 
 def tensor_spec(name: str, dtype: str, shape, optional: bool = False) -> tuple:
-    """One argument of an executable: its name, dtype, shape (a tuple, or an int: that many elements), whether it may be None."""
+    """One argument of an executable: its name, dtype, shape (a tuple, or an int: that many elements, -1: any number), whether
+    it may be None."""
     import torch
 
     return name, getattr(torch, dtype), shape, optional
@@ -116,10 +117,7 @@ _torch = None
 
 
 def require_tensors(specs, tensors) -> int:
-    """ValueError unless every tensor is what its spec says, contiguous and on the current device; returns that device.
-
-    On the launch path of calls that take ten microseconds on the GPU: one pass over plain attributes, and the search for
-    what is wrong only when something is."""
+    """ValueError unless every tensor is what its spec says, contiguous and on the current device; returns that device."""
     global _torch
     if _torch is None:
         import torch
@@ -132,7 +130,7 @@ def require_tensors(specs, tensors) -> int:
             continue
         try:
             if (t.dtype is dtype and t.get_device() == device and t.is_contiguous()
-                    and (t.shape == shape if shape.__class__ is tuple else t.numel() == shape)):
+                    and (t.shape == shape if shape.__class__ is tuple else shape < 0 or t.numel() == shape)):
                 continue
         except AttributeError:
             pass
@@ -150,7 +148,7 @@ def _refuse(spec, t, device: int):
         raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
     if isinstance(shape, tuple) and tuple(t.shape) != shape:
         raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
-    if isinstance(shape, int) and t.numel() != shape:
+    if isinstance(shape, int) and 0 <= shape != t.numel():
         raise ValueError(f"{name} must have {shape} elements, got {t.numel()}")
     if not t.is_cuda:
         raise ValueError(f"{name}: all tensors must be CUDA tensors")

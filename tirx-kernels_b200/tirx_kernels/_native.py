@@ -1,4 +1,4 @@
-"""ctypes binding of the C-ABI library (include/b200_nvfp4.h).
+"""ctypes binding of the C-ABI library (include/b200_nvfp4.h), and the compiled binding of the operators' calls (`Launch`).
 
 The library is the product: if it is missing or a symbol cannot be resolved, import of a
 kernel module fails loudly.  Nothing here falls back to PyTorch or CPU code.
@@ -7,6 +7,8 @@ kernel module fails loudly.  Nothing here falls back to PyTorch or CPU code.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 from pathlib import Path
 
@@ -25,6 +27,7 @@ OK, ERR_INVALID_ARGUMENT, ERR_CUDA, ERR_DEVICE_TIMEOUT, ERR_UNSUPPORTED = range(
 _LIB_DIR = Path(__file__).resolve().parent.parent / "lib"
 _MAIN = None
 _CUBLASLT = None
+_BINDING = None
 
 _vp, _i, _f, _i64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_int64
 
@@ -233,7 +236,51 @@ def nvfp4_gemm_small_m_noalloc(A, B, SFA, SFB, alpha, D, M: int, N: int, K: int)
     )
 
 
-# ---- the feed-forward operators: checked argument by argument in their modules (_checks.require_tensors) ----
+# ---- the feed-forward operators: checked argument by argument against the specs of their modules ----
+def _binding():
+    global _BINDING
+    if _BINDING is None:
+        import torch  # noqa: F401  (the libraries that the binding is linked to)
+
+        path = _LIB_DIR / "b200nvfp4_binding.so"
+        if not path.exists():
+            raise NativeLibraryError(f"{path} not found: build it with `python tirx-kernels_b200/build.py`")
+        loader = importlib.machinery.ExtensionFileLoader("b200nvfp4_binding", str(path))
+        _BINDING = importlib.util.module_from_spec(importlib.util.spec_from_loader(loader.name, loader))
+        loader.exec_module(_BINDING)
+    return _BINDING
+
+
+class Launch:
+    """An entry point with the specs of its tensors (_checks.tensor_spec) and its sizes (None: given with each call).
+
+    Called with the tensors and what is given, it checks them, launches on the current stream of the current device and
+    raises what is wrong.  Without a symbol it is the check alone."""
+
+    __slots__ = ("symbol", "specs", "sizes", "bound")
+
+    def __init__(self, symbol, specs, sizes=()):
+        self.symbol, self.specs, self.sizes, self.bound = symbol, specs, sizes, None
+
+    def __call__(self, *args) -> None:
+        status = (self.bound or self._bind())(*args)
+        if status:
+            self._fail(status, args)
+
+    def _bind(self):
+        address = ctypes.cast(getattr(lib(), self.symbol), ctypes.c_void_p).value if self.symbol else 0
+        self.bound = _binding().bind(self.symbol, address, self.specs, self.sizes)
+        return self.bound
+
+    def _fail(self, status, args):
+        if status > 0:
+            check(status, self.symbol)
+        from tirx_kernels import _checks
+
+        _checks.require_tensors(self.specs, args[:len(self.specs)])
+        raise ValueError(f"{self.symbol}: tensors refused")
+
+
 def call(symbol: str, device: int, tensors, *sizes) -> None:
     """`symbol` of `tensors` as their addresses (None as null) and `sizes`, on the current stream of `device`, the current device."""
     import torch

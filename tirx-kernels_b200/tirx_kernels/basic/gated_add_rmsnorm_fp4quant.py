@@ -37,18 +37,15 @@ class _Executable:
             spec("gate", input_dtype, (_checks.ceil_div(M, rows_per_gate), H), True), spec("w_pre", input_dtype, (H,)),
             spec("residual_out", *rows), spec("y", "uint8", (M, H // 2)) if quantize else spec("y", *rows),
         )
-        if quantize:
-            self.specs += (spec("sf", "uint8", _checks.sf_numel(M, H // 16, "128x4" if swizzled else "linear")),
-                           spec("global_scale", "float32", 1))
-        self.sizes = M, H, rows_per_gate
-        self.codes = _native.DTYPE_CODES[input_dtype], int(bool(quantize)), int(bool(swizzled))
+        sf = _checks.sf_numel(M, H // 16, "128x4" if swizzled else "linear") if quantize else -1
+        self.specs += (spec("sf", "uint8", sf, not quantize), spec("global_scale", "float32", 1, not quantize))
+        self.launch = _native.Launch("b2_gated_add_rmsnorm_fp4quant", self.specs, (
+            M, H, rows_per_gate, None, None, _native.DTYPE_CODES[input_dtype], int(self.quantize), int(bool(swizzled))))
 
     def __call__(self, x, residual, w_post, gate, w_pre, residual_out, y, sf, global_scale, residual_scale: float, eps: float) -> None:
         if not self.quantize and (sf is not None or global_scale is not None):
             raise ValueError("sf and global_scale belong to the quantized form")
-        tensors = x, residual, w_post, gate, w_pre, residual_out, y, sf, global_scale
-        _native.call("b2_gated_add_rmsnorm_fp4quant", _checks.require_tensors(self.specs, tensors), tensors, *self.sizes,
-                     residual_scale, eps, *self.codes)
+        self.launch(x, residual, w_post, gate, w_pre, residual_out, y, sf, global_scale, residual_scale, eps)
 
 
 def get_kernel(input_dtype: str, M: int, H: int, quantize: bool = True, swizzled: bool = True, rows_per_gate: int = 1, **kwargs) -> KernelHandle:

@@ -33,13 +33,20 @@ def _weight_specs(experts: int, inner: int, hidden: int) -> tuple:
             spec("sf2", "uint8", experts * _checks.sf_numel(hidden, inner // 16, "128x4")), scalars("alpha2"), scalars("gs2"))
 
 
+@functools.lru_cache(maxsize=64)
+def _weight_check(experts: int, inner: int, hidden: int):
+    return _native.Launch(None, _weight_specs(experts, inner, hidden))
+
+
 @functools.lru_cache(maxsize=256)
-def _call_specs(tokens: int, topk: int, experts: int, hidden: int, inner: int, dtype: str) -> tuple:
-    """(argument specs of expert_ffn, workspace bytes) of a shape."""
+def _ffn_launch(tokens: int, topk: int, experts: int, hidden: int, inner: int, dtype: str) -> tuple:
+    """(launch, workspace bytes) of a shape."""
     spec = _checks.tensor_spec
     rows = dtype, (tokens, hidden)
-    return ((spec("x", *rows), spec("ids", "int32", (tokens, topk)), spec("gates", "float32", (tokens, topk)),
-             spec("residual", *rows, True), spec("out", *rows)), workspace_bytes(tokens, topk, experts, hidden, inner))
+    specs = (spec("x", *rows), spec("ids", "int32", (tokens, topk)), spec("gates", "float32", (tokens, topk)),
+             *_weight_specs(experts, inner, hidden), spec("residual", *rows, True), spec("out", *rows), spec("workspace", "uint8", -1))
+    size = workspace_bytes(tokens, topk, experts, hidden, inner)
+    return _native.Launch("b2_moe_expert_ffn", specs, (None, tokens, topk, experts, hidden, inner, _native.DTYPE_CODES[dtype])), size
 
 
 @dataclass(frozen=True)
@@ -64,8 +71,8 @@ class ExpertWeights:
         if getattr(self.w1, "ndim", 0) != 3 or getattr(self.w2, "ndim", 0) != 3 or self.w1.shape[1] % 2:
             raise ValueError("w1 and w2 must be [experts, 2 * inner, hidden / 2] and [experts, hidden, inner / 2]")
         (experts, gate_up, half) = self.w1.shape
-        _checks.require_tensors(_weight_specs(experts, gate_up // 2, half * 2),
-                                (self.w1, self.sf1, self.alpha1, self.gs1, self.w2, self.sf2, self.alpha2, self.gs2))
+        _weight_check(experts, gate_up // 2, half * 2)(self.w1, self.sf1, self.alpha1, self.gs1, self.w2, self.sf2, self.alpha2,
+                                                       self.gs2)
 
     @property
     def experts(self) -> int:
@@ -190,21 +197,15 @@ def expert_ffn(x, ids, gates, weights: ExpertWeights, *, residual=None, out=None
     tokens, topk = ids.shape
     sizes = tokens, topk, *weights.w2.shape[:2], weights.w2.shape[2] * 2
     dtype = _operator.dtype_name(x.dtype)
-    specs, size = _call_specs(*sizes, dtype)
+    launch, size = _ffn_launch(*sizes, dtype)
     if out is None:
         out = torch.empty_like(x)
-    device = _checks.require_tensors(specs, (x, ids, gates, residual, out))
     if workspace is None:
         workspace = torch.empty(size, dtype=torch.uint8, device=x.device)
-    elif (workspace.dtype != torch.uint8 or workspace.numel() < size or workspace.get_device() != device
-          or not workspace.is_contiguous()):
-        raise ValueError(f"workspace must be contiguous uint8 on cuda:{device} with at least {size} elements, got "
-                         f"{workspace.numel()} of {workspace.dtype} on {workspace.device}")
-    if weights.w1.get_device() != device:
-        raise ValueError(f"weights are on {weights.w1.device}, but the current device is cuda:{device}")
-    _native.call("b2_moe_expert_ffn", device,
-                 (x, ids, gates, weights.w1, weights.sf1, weights.alpha1, weights.gs1, weights.w2, weights.sf2, weights.alpha2,
-                  weights.gs2, residual, out, workspace), workspace.numel(), *sizes, _native.DTYPE_CODES[dtype])
+    elif workspace.numel() < size:
+        raise ValueError(f"workspace must have at least {size} elements, got {workspace.numel()}")
+    w = weights
+    launch(x, ids, gates, w.w1, w.sf1, w.alpha1, w.gs1, w.w2, w.sf2, w.alpha2, w.gs2, residual, out, workspace, workspace.numel())
     return out
 
 

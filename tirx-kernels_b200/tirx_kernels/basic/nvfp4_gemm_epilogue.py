@@ -40,11 +40,11 @@ class _Runner:
             spec("alpha", "float32", 1), spec("bias", out_dtype, (N,), True), spec("residual", out_dtype, (M, N), True),
             spec("D", out_dtype, (M, N)),
         )
-        self.sizes = M, N, K, _native.DTYPE_CODES[out_dtype], _native.ACTIVATION_CODES[activation]
+        self.launch = _native.Launch("b2_nvfp4_gemm_epilogue", self.specs, (M, N, K, _native.DTYPE_CODES[out_dtype],
+                                                                       _native.ACTIVATION_CODES[activation]))
 
     def __call__(self, A, B, SFA, SFB, alpha, bias, residual, D) -> None:
-        tensors = A, B, SFA, SFB, alpha, bias, residual, D
-        _native.call("b2_nvfp4_gemm_epilogue", _checks.require_tensors(self.specs, tensors), tensors, *self.sizes)
+        self.launch(A, B, SFA, SFB, alpha, bias, residual, D)
 
 
 def get_kernel(M: int, N: int, K: int, activation: str = "none", out_dtype: str = "bfloat16", **kwargs) -> KernelHandle:

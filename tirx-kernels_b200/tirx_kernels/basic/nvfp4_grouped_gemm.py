@@ -37,11 +37,11 @@ class _Runner:
             spec("SFB", "uint8", groups * _checks.sf_numel(N, K // 16, "128x4")), spec("alpha", "float32", (groups,)),
             spec("offsets", "int32", (groups + 1,)), spec("bias", out_dtype, (groups, N), True), spec("D", out_dtype, (rows, N)),
         )
-        self.sizes = rows, groups, N, K, _native.DTYPE_CODES[out_dtype], _native.ACTIVATION_CODES[activation]
+        self.launch = _native.Launch("b2_nvfp4_grouped_gemm", self.specs, (rows, groups, N, K, _native.DTYPE_CODES[out_dtype],
+                                                                      _native.ACTIVATION_CODES[activation]))
 
     def __call__(self, A, B, SFA, SFB, alpha, offsets, bias, D) -> None:
-        tensors = A, B, SFA, SFB, alpha, offsets, bias, D
-        _native.call("b2_nvfp4_grouped_gemm", _checks.require_tensors(self.specs, tensors), tensors, *self.sizes)
+        self.launch(A, B, SFA, SFB, alpha, offsets, bias, D)
 
 
 def get_kernel(rows: int, groups: int, N: int, K: int, activation: str = "none", out_dtype: str = "bfloat16", **kwargs) -> KernelHandle:

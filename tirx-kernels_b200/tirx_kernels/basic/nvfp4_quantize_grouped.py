@@ -35,11 +35,11 @@ class _Executable:
             spec("offsets", "int32", (groups + 1,)), spec("out", "uint8", (rows, k // 2)),
             spec("sf", "uint8", _checks.grouped_sf_numel(rows, groups, k)), spec("global_scale", "float32", (groups,)),
         )
-        self.sizes = in_rows, rows, groups, k, _native.DTYPE_CODES[dtype], int(fuse_silu)
+        self.launch = _native.Launch("b2_nvfp4_quantize_grouped", self.specs, (in_rows, rows, groups, k, _native.DTYPE_CODES[dtype],
+                                                                          int(fuse_silu)))
 
     def __call__(self, x, index, offsets, out, sf, global_scale) -> None:
-        tensors = x, index, offsets, out, sf, global_scale
-        _native.call("b2_nvfp4_quantize_grouped", _checks.require_tensors(self.specs, tensors), tensors, *self.sizes)
+        self.launch(x, index, offsets, out, sf, global_scale)
 
 
 def get_kernel(dtype: str, in_rows: int, rows: int, groups: int, k: int, fuse_silu: bool = False, **kwargs) -> KernelHandle:
