@@ -61,6 +61,14 @@ def quantize_weights(w):
     return torch.stack([p for p, _ in parts]), torch.cat([s for _, s in parts]), gs
 
 
+def _uneven(rows: int, groups: int, generator):
+    """Offsets of `groups` groups cut at random places."""
+    import torch
+
+    cuts = torch.randint(0, rows + 1, (groups - 1,), generator=generator).sort().values
+    return torch.cat([torch.zeros(1, dtype=torch.long), cuts, torch.tensor([rows])])
+
+
 def prepare_data(rows: int, groups: int, N: int, K: int, out_dtype: str = "bfloat16", bias: bool = True, sizes=None, **kwargs):
     """Seeded (A, B, SFA, SFB, alpha, offsets, bias); `sizes` rows per group, else uneven groups, some of them empty."""
     import torch
@@ -70,8 +78,7 @@ def prepare_data(rows: int, groups: int, N: int, K: int, out_dtype: str = "bfloa
     generator = torch.Generator().manual_seed(1)
     draw = lambda *shape: torch.randn(*shape, generator=generator)
     if sizes is None:
-        cuts = torch.randint(0, rows + 1, (groups - 1,), generator=generator).sort().values
-        offsets = torch.cat([torch.zeros(1, dtype=torch.long), cuts, torch.tensor([rows])])
+        offsets = _uneven(rows, groups, generator)
     else:
         offsets = torch.cat([torch.zeros(1, dtype=torch.long), torch.tensor(list(sizes)).cumsum(0)])
     offsets = offsets.to(torch.int32).cuda()
@@ -131,8 +138,11 @@ def flops(rows: int, N: int, K: int) -> int:
 
 
 def algorithmic_bytes(rows: int, groups: int, N: int, K: int) -> int:
-    """With every group's weight touched (an upper bound when there are few rows)."""
-    return rows * K * 9 // 16 + min(groups, rows) * N * K * 9 // 16 + rows * N * 2
+    """Operands, the weights of the groups that have rows (of `prepare_data`'s uneven ones) and the output."""
+    import torch
+
+    touched = int((_uneven(rows, groups, torch.Generator().manual_seed(1)).diff() > 0).sum())
+    return rows * K * 9 // 16 + touched * N * K * 9 // 16 + rows * N * 2
 
 
 def _make_launch(rows, groups, N, K, activation="none", out_dtype="bfloat16", bias=True, sizes=None):
