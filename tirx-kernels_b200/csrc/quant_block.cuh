@@ -16,6 +16,53 @@ __device__ __forceinline__ uint32_t silu_and_mul_pair(uint32_t gate, uint32_t up
   return pack_from_f32<Tag>(s.x, s.y);
 }
 
+// The same for four pairs side by side: silu_f32x2 with one choice of path for all of them, so that their chains of
+// dependent instructions overlap.
+template <typename Tag>
+__device__ __forceinline__ void silu_and_mul_4(const uint32_t (&gate)[4], const uint32_t (&up)[4], uint32_t (&out)[4]) {
+  const float2 one = make_float2(1.0f, 1.0f), minus = make_float2(-1.0f, -1.0f);
+  const float2 log2e = make_float2(-1.4426950408889634f, -1.4426950408889634f);
+  constexpr float kTiny = 8.67361737988e-19f;  // 2^-60
+  float2 g[4], e[4], s[4];
+  bool fast = true;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    g[i] = unpack2<Tag>(gate[i]);
+    const float2 t = mul_f32x2(g[i], log2e);
+    e[i] = make_float2(ex2_approx_ftz(t.x), ex2_approx_ftz(t.y));
+    fast = fast && fmaxf(fabsf(t.x), fabsf(t.y)) < 64.0f && fabsf(g[i].x) >= kTiny && fabsf(g[i].y) >= kTiny;
+  }
+  if (fast) {
+    float2 nd[4], r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 d = fma_f32x2(e[i], one, one);
+      nd[i] = fma_f32x2(e[i], minus, minus);
+      r[i] = make_float2(rcp_approx_ftz(d.x), rcp_approx_ftz(d.y));
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = fma_f32x2(r[i], fma_f32x2(nd[i], r[i], one), r[i]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = mul_f32x2(g[i], r[i]);
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[i] = fma_f32x2(fma_f32x2(nd[i], s[i], g[i]), r[i], s[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 d = fma_f32x2(e[i], one, one);
+      s[i] = make_float2(__fdiv_rn(g[i].x, d.x), __fdiv_rn(g[i].y, d.y));
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 m = mul_f32x2(s[i], unpack2<Tag>(up[i]));
+    out[i] = pack_from_f32<Tag>(m.x, m.y);
+  }
+}
+
 // One 16-element block held as 8 packed words -> (E4M3 scale byte, 64 packed E2M1 bits).
 template <typename Tag>
 __device__ __forceinline__ void quantize_block(const uint32_t (&w)[8], float gs, float rcp_gs,
