@@ -200,6 +200,16 @@ def test_grouped_many_groups_and_tiles(variant):
         mod.run_test(2000, 3, 4104, 64, bias=False)
 
 
+@pytest.mark.parametrize("K", [960, 1024, 1088, 2048])
+@pytest.mark.parametrize("activation,out_dtype", [("none", "bfloat16"), ("gelu", "float16")])
+def test_grouped_few_rows_on_both_sides_of_the_split_epilogue(K, activation, out_dtype, variant):
+    from tirx_kernels.basic import nvfp4_grouped_gemm as mod
+
+    variant(1)
+    mod.run_test(230, 12, 328, K, activation, out_dtype, True, sizes=[0, 1, 32, 33, 64, 7, 0, 31, 2, 60, 0, 0])
+    mod.run_test(40, 40, 4096, K, bias=False, sizes=[1] * 40)
+
+
 @pytest.mark.parametrize("which", [1, 3, 4])
 def test_grouped_more_row_tiles_than_are_mapped(which, variant):
     """Behind the row tiles whose group is looked up (512 of single CTAs, 128 of pairs) it is searched."""

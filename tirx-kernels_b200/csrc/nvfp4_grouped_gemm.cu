@@ -326,6 +326,7 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
   constexpr uint32_t kScaleTx = static_cast<uint32_t>(L::kSfaBytes + L::kSfbBytes);
   constexpr bool kWarpWide = CG == 2;  // issuing roles run as whole warps (see nvfp4_gemm.cu)
   constexpr int kCols = BN / PARTS;    // columns of an epilogue warp
+  constexpr int kOuts = kCols / 2;     // gated: its outputs
   constexpr int kWarpEpi0 = kGWarpScale0 + 4 * SETS;
   constexpr bool kMoveRegisters = PARTS == 4;
   static_assert((kCols == 32 || kCols == 64) && (!kMoveRegisters || SETS == 1), "epilogue shapes");
@@ -821,15 +822,15 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
         const uint32_t here = buffers + static_cast<uint32_t>(lane >> 4) * 2048u + (lane & 15) * 128u;
         const float gs = MODE == kGated ? __ldg(p.gs + w.tile.group) : 0.0f;
 #pragma unroll 1
-        for (int c0 = 0; c0 < (MODE == kGated ? 32 : kCols); c0 += 16) {
+        for (int c0 = 0; c0 < (MODE == kGated ? kOuts : kCols); c0 += 16) {
           uint32_t v[16];
           if constexpr (MODE == kGated) {
             uint32_t up[16];
-            tmem_ld_32x16(acc_tmem + part * 32 + c0, v);
-            tmem_ld_32x16(acc_tmem + BN / 2 + part * 32 + c0, up);
+            tmem_ld_32x16(acc_tmem + part * kOuts + c0, v);
+            tmem_ld_32x16(acc_tmem + BN / 2 + part * kOuts + c0, up);
             tmem_ld_wait();
             if (w.mine) {
-              const int col = w.tile.tn * (BN / 2) + part * 32 + c0;
+              const int col = w.tile.tn * (BN / 2) + part * kOuts + c0;
               uint32_t sf_byte;
               uint2 packed;
               if (p.fp16) gated_block<F16Tag, true>(v, up, w.alpha, gs, sf_byte, packed);
@@ -1220,7 +1221,12 @@ int run_dense(int variant, const GroupedCall& c, cudaStream_t s) {
 int run_groups(int variant, const GroupedCall& c, cudaStream_t s) {
   switch (variant) {
     case 0:
-    case 1: return launch_grouped<kGrouped, 1, 128, 8, 0, 32, 1, 2>(c, s);
+    case 1:
+      // Of a 32-row tile only the epilogue warps of the first lane quarter have rows.  Where a tile has few slabs they are
+      // what it waits for: twice as many parts, with half of the columns each (40 groups of one row, N = 4096: K = 512
+      // 14.7 us for 17.8, K = 1024 18.0 for 19.7; K = 2048 34.4 for 33.6, with one set of scale warps).
+      if (c.K <= 1024) return launch_grouped<kGrouped, 1, 128, 8, 0, 32, 1, 2, 1, 4>(c, s);
+      return launch_grouped<kGrouped, 1, 128, 8, 0, 32, 1, 2>(c, s);
     case 2:
     case 3: return launch_grouped<kGrouped, 1, 128, 5, 1, 128, 1, 2>(c, s);
     case 4: return launch_grouped<kGrouped, 2, 256, 5, 1, 128, 1, 1, 1, 4>(c, s);
