@@ -304,3 +304,36 @@ def test_bound_calls_refuse_what_they_are_not_made_for():
         check(a, b=None)
     with pytest.raises(ValueError, match="a: all tensors must be CUDA"):
         _native.Launch(None, (spec("a", "float32", (2, 3)),))(a)
+
+
+@pytest.mark.parametrize("stages,issuers,safe", [(3, 1, True), (4, 1, True), (2, 2, True), (4, 2, True), (6, 2, True), (3, 2, False), (5, 2, False)])
+def test_ring_of_two_issuers_is_even(stages, issuers, safe):
+    """All orders in which slabs land and are consumed: a wait by phase parity never passes for a slab that has not landed.
+
+    Slab n lies in stage n % stages, its load is issued when the slab before it in that stage was consumed, loads land in any
+    order, issuer n % issuers consumes slab n when the parity test of the stage's barrier passes: phases completed there and
+    the phase asked for, n // stages, differ in parity, or (the stale case) the test sees the phase in front of an open one."""
+    slabs = 3 * stages
+    seen, todo = set(), [(0, tuple(range(issuers)))]  # bit mask of landed slabs, next slab of every issuer
+    stale = False
+    while todo and not stale:
+        state = todo.pop()
+        if state in seen:
+            continue
+        seen.add(state)
+        landed, heads = state
+        consumed = lambda n: n < heads[n % issuers]
+        issued = 0
+        while issued < slabs and (issued < stages or consumed(issued - stages)):
+            issued += 1  # in order
+        for n in range(issued):
+            if not landed >> n & 1:
+                todo.append((landed | 1 << n, heads))
+        for i, n in enumerate(heads):
+            if n >= slabs:
+                continue
+            completed = sum(landed >> m & 1 for m in range(n % stages, slabs, stages))  # phases of the stage's barrier
+            if completed % 2 != n // stages % 2:
+                stale = stale or not landed >> n & 1
+                todo.append((landed, heads[:i] + (n + issuers,) + heads[i + 1:]))
+    assert stale != safe

@@ -99,6 +99,10 @@ __global__ void __launch_bounds__(kThreads + 32 * (MMAS - 1), 1)
   using L = SmemLayout<CG, BN, STAGES, TMA_OUT, AM>;
   static_assert(MMAS == 1 || (MMAS == 2 && CG == 1 && TMA_OUT == 0), "the second MMA warp exists for single-CTA tiles");
   static_assert(BN * MMAS + STAGES * L::kSfCols <= 512, "tensor memory budget");
+  // A stage's slabs belong to one issuer then.  With an odd ring the other issuer may still wait for the stage's last slab
+  // when this one polls for the next: the parity of the phase in front of that slab's is the one it asks for, and it would
+  // take the poll for its own slab's.
+  static_assert(STAGES % MMAS == 0, "two issuers need an even ring");
   constexpr int kAccCols = BN * MMAS;  // accumulator columns in front of the stages' scale areas
   constexpr int kWarpMma2 = 19;
   constexpr int kTmemCols = 512;
@@ -1074,8 +1078,8 @@ extern "C" int b2_nvfp4_gemm(const void* A, const void* B, const void* SFA, cons
     case 4: return launch_variant<1, 128, 9, 0, 32>(A, B, SFA, SFB, alpha_dev, D, M, N, K, 4, s);
     case 5: return launch_variant<1, 256, 5, 0, 32>(A, B, SFA, SFB, alpha_dev, D, M, N, K, 5, s);
     case 6: return launch_variant<1, 64, 13, 0, 32>(A, B, SFA, SFB, alpha_dev, D, M, N, K, 6, s);
-    case 7: return launch_variant<1, 64, 11, 0, 32, 2>(A, B, SFA, SFB, alpha_dev, D, M, N, K, 7, s);
-    case 8: return launch_variant<1, 64, 7, 0, 128, 2>(A, B, SFA, SFB, alpha_dev, D, M, N, K, 8, s);
+    case 7: return launch_variant<1, 64, 12, 0, 32, 2>(A, B, SFA, SFB, alpha_dev, D, M, N, K, 7, s);
+    case 8: return launch_variant<1, 64, 8, 0, 128, 2>(A, B, SFA, SFB, alpha_dev, D, M, N, K, 8, s);
     case 9: return launch_variant<1, 128, 6, 0, 128, 2>(A, B, SFA, SFB, alpha_dev, D, M, N, K, 9, s);
     default: return launch_variant<2, 128, 6, 1>(A, B, SFA, SFB, alpha_dev, D, M, N, K, 3, s);
   }
@@ -1219,8 +1223,8 @@ extern "C" int b2_nvfp4_gemm_small_m_noalloc(const void* A, const void* B, const
     case 0: return launch_variant<1, 128, 6>(A, B, SFA, SFB, alpha_dev, D, M, N, K, 0, s, &ws);
     case 1: return launch_variant<1, 256, 4>(A, B, SFA, SFB, alpha_dev, D, M, N, K, 1, s, &ws);
     case 4: return launch_variant<1, 128, 9, 0, 32>(A, B, SFA, SFB, alpha_dev, D, M, N, K, 4, s, &ws);
-    case 7: return launch_variant<1, 64, 11, 0, 32, 2>(A, B, SFA, SFB, alpha_dev, D, M, N, K, 7, s, &ws);
-    case 8: return launch_variant<1, 64, 7, 0, 128, 2>(A, B, SFA, SFB, alpha_dev, D, M, N, K, 8, s, &ws);
+    case 7: return launch_variant<1, 64, 12, 0, 32, 2>(A, B, SFA, SFB, alpha_dev, D, M, N, K, 7, s, &ws);
+    case 8: return launch_variant<1, 64, 8, 0, 128, 2>(A, B, SFA, SFB, alpha_dev, D, M, N, K, 8, s, &ws);
     default: return launch_variant<1, 256, 5, 0, 32>(A, B, SFA, SFB, alpha_dev, D, M, N, K, 5, s, &ws);
   }
 }

@@ -317,6 +317,10 @@ __global__ void __launch_bounds__(group_threads(SETS, PARTS), 1)
   using L = GroupedLayout<MODE, CG, BN, STAGES, TMA_OUT, AM>;
   static_assert(MMAS == 1 || (CG == 1 && TMA_OUT == 0), "the second MMA warp exists for single-CTA tiles");
   static_assert(CG == 1 || AM == kBlockM, "pairs load all rows");
+  // A stage's slabs belong to one issuer then.  With an odd ring the other issuer may still wait for the stage's last slab
+  // when this one polls for the next: the parity of the phase in front of that slab's is the one it asks for, and it would
+  // take the poll for its own slab's.
+  static_assert(STAGES % MMAS == 0, "two issuers need an even ring");
   constexpr int kBM = AM * CG;                // rows of a tile
   constexpr int kAccCols = BN * MMAS * NACC;  // accumulator columns in front of the stages' scale areas
   static_assert(kAccCols + STAGES * L::kSfCols <= 512, "tensor memory budget");
@@ -1210,9 +1214,9 @@ int choose_grouped_variant(int rows, int groups, bool grouped, int N, int K, int
 // 128 x 128 tiles holds one more scale chunk (five stages for six), and pairs take 256 columns: 128 gates, 128 ups.
 int run_dense(int variant, const GroupedCall& c, cudaStream_t s) {
   switch (variant) {
-    case 0: return launch_grouped<kDense, 1, 64, 11, 0, 32, 2, 1>(c, s);
+    case 0: return launch_grouped<kDense, 1, 64, 12, 0, 32, 2, 1>(c, s);
     case 1: return launch_grouped<kDense, 1, 128, 8, 0, 32, 1, 2>(c, s);
-    case 2: return launch_grouped<kDense, 1, 64, 7, 0, 128, 2, 1>(c, s);
+    case 2: return launch_grouped<kDense, 1, 64, 8, 0, 128, 2, 1>(c, s);
     case 3: return launch_grouped<kDense, 1, 128, 5, 1, 128, 1, 2>(c, s);
     case 4: return launch_grouped<kDense, 2, 256, 5, 1, 128, 1, 1, 1, 4>(c, s);
     default: return launch_grouped<kDense, 2, 128, 6, 1, 128, 1, 2>(c, s);
