@@ -1181,13 +1181,13 @@ std::atomic<int> g_grouped_variant{-1};  // test hook: -1 = automatic
 
 // The kernel for `rows` rows in `groups` groups (numbering of b2_nvfp4_grouped_gemm_set_variant).  Times on B200, back
 // to back launches from a CUDA graph, us:
-//   dense     32 x 64, 2 MMA warps   all of N in one wave of 64-wide tiles: 16 x 8192 x 8192 10.4 (32 x 128: 12.4)
-//             32 x 128               more: 16 x 28672 x 8192 25.8 (32 x 64: 35.5)
-//             128 x 64, 2 MMA warps  one wave of them: 1024^3 4.8 (128 x 128: 6.0, 256 x 128: 6.1), 200 x 4096 x 4096 7.1 (9.0, 8.4)
-//             128 x 128              more columns, at most 128 rows: 64 x 28672 x 8192 28.1 (256 x 256: 32.3), or K up to 2048
+//   dense     32 x 64, 2 MMA warps   all of N in one wave of 64-wide tiles: 16 x 8192 x 8192 10.2 (32 x 128: 11.4)
+//             32 x 128               more: 16 x 28672 x 8192 24.4 (32 x 64: 31.8)
+//             128 x 64, 2 MMA warps  one wave of them: 1024^3 4.3 (128 x 128: 5.1, 256 x 128: 5.3), 200 x 4096 x 4096 6.6 (8.1, 7.2)
+//             128 x 128              more columns, at most 128 rows: 64 x 28672 x 8192 27.2 (256 x 256: 31.2), or K up to 2048
 //                                    and one wave: 1000 x 2048 x 2048 6.1 (256 x 128: 6.7; at K = 4096 both 8.2)
-//             256 x 128              one wave of them: 256 x 8192 x 8192 10.9 (256 x 256: 16.2, 128 x 128: 12.4)
-//             256 x 256              the rest: 2048 x 4096 x 4096 19.3 (256 x 128: 20.4)
+//             256 x 128              one wave of them: 256 x 8192 x 8192 11.1 (256 x 256: 15.2, 128 x 128: 12.7)
+//             256 x 256              the rest: 2048 x 4096 x 4096 18.7 (256 x 128: 19.7)
 //   grouped   32 x 128               mean of 16 rows: 1024 rows of 64, N=2048, K=4096 55.3 (128 x 128: 56.1); 8 rows,
 //                                    N=4096, K=2048 11.1 (14.3)
 //             128 x 128              mean of 64 rows: 4096 of 64, N=K=2048 36.5 (256 x 256: 39.3), or about one wave of
