@@ -708,3 +708,30 @@ def test_bound_calls_check_every_tensor_and_follow_stream_and_numbers():
         ex(late, residual, w_post, gate, w_pre, h, y, None, None, 1.0, 1e-6)  # behind the copy, on its stream
     stream.synchronize()
     assert torch.equal(h, want)
+
+
+@pytest.mark.parametrize("M,N,K,which", [(236, 144, 4928, 2), (16, 2048, 4864, 0), (30, 320, 2624, 0), (500, 200, 7104, 2)])
+def test_two_issuers_beside_another_stream(M, N, K, which, variant):
+    """Tiles with two MMA-issuing warps while another stream's kernels slow some of their warps: the same bits every time."""
+    from tirx_kernels import _native
+    from tirx_kernels.basic import gated_add_rmsnorm_fp4quant as norm, nvfp4_gemm_epilogue as mod
+
+    variant(which)
+    data = mod.prepare_data(M, N, K, residual=False)
+    ex = _launcher(mod, M=M, N=N, K=K, activation="gelu_tanh")
+    x, residual, w_post, gate, w_pre, _ = norm.prepare_data("bfloat16", 700, 1024)
+    nex = _launcher(norm, input_dtype="bfloat16", M=700, H=1024, quantize=False)
+    h, y = torch.empty_like(x), torch.empty_like(x)
+    want = torch.empty(M, N, dtype=torch.bfloat16, device="cuda")
+    ex(*data, want)
+    outs = torch.empty(400, M, N, dtype=torch.bfloat16, device="cuda")
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for out in outs:
+        with torch.cuda.stream(streams[0]):
+            ex(*data, out)
+        with torch.cuda.stream(streams[1]):
+            nex(x, residual, w_post, gate, w_pre, h, y, None, None, 1.0, 1e-6)
+    torch.cuda.synchronize()
+    _native.nvfp4_grouped_gemm_status()
+    assert (outs == want).all()
